@@ -1,0 +1,240 @@
+// quant_kv.hip — a key/value cache in 8 or 4 bits (chronos_quant_kv.h has its layout): written from a projection's rows in one pass, and read back.
+//
+// norm_rope_kv_quant.  qkv[T, (Hq + 2 Hkv) D], per head row x:
+//   y = x / sqrt(mean(x^2) + eps) * w     queries and keys that have weights
+//   y1' = y1 c - y2 s, y2' = y2 c + y1 s  queries and keys, the first R dimensions in two halves, c, s = cos_sin[pos, : R / 2], cos_sin[pos, R / 2 :]
+//   q = y' in bfloat16; k = y', v = x in the cache's codes and scales, at block_table[tok_seq, pos / page], row pos % page.
+// It reads T (Hq + 2 Hkv) D 2 bytes and writes T Hq D 2 and the rows' codes: bytes are what bounds it.  D / 8 lanes a head row, 16 bytes a lane; a lane's rotation
+// partner is D / 16 lanes away or none, and its eight numbers are read a second time (they are in the cache) where an exchange would go through LDS.  Keys and values
+// go by double up to their codes: a key next to a border between two codes then takes the code of the formula, whatever the order of sums, and it costs nothing
+// beside the bytes.  Queries are float32 but for their sum of squares.
+#include "chronos_quant_kv.h"
+
+namespace chronos {
+namespace qkv {
+namespace {
+
+// over n neighbouring lanes, n = 4, 8 or 16, all of them active
+template <int CTRL> __device__ __forceinline__ double dpp(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int n, typename Op> __device__ __forceinline__ double group_all(double v, Op&& op) {
+    v = op(v, dpp<0xb1>(v));                      // quad_perm 1 0 3 2
+    v = op(v, dpp<0x4e>(v));                      // quad_perm 2 3 0 1
+    if constexpr (n > 4) v = op(v, dpp<0x141>(v));   // row_half_mirror
+    if constexpr (n > 8) v = op(v, dpp<0x140>(v));   // row_mirror
+    return v;
+}
+struct Sum { __device__ double operator()(double a, double b) const { return a + b; } };
+struct Max { __device__ double operator()(double a, double b) const { return fmax(a, b); } };
+
+__device__ __forceinline__ void ld8(const uint16_t* p, float (&v)[8]) {
+    const u16x8 r = *reinterpret_cast<const u16x8*>(p);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = bf2f(r[j]);
+}
+
+// Eight numbers of a row into its codes; lane c of the row's D / 8 (all active).  `there`: the row has a place.
+template <int KIND, int D> __device__ __forceinline__ void put(const double (&y)[8], int c, bool there, uint8_t* codes, void* scales, int64_t row) {
+    constexpr double kInf = __builtin_huge_val();
+    double top = 0.;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmax(top, fabs(y[j]) < kInf ? fabs(y[j]) : kInf);   // NaN counts as an infinity
+    if constexpr (KIND == kInt8) {
+        top = group_all<D / 8>(top, Max{});
+        const bool whole = top < kInf;
+        const float s = whole ? (float)(top / 127.) : __builtin_nanf("");
+        const double inv = s > 0.f ? 1. / (double)s : 0.;
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int n = inv > 0. ? (int)fmin(fmax(rint(y[j] * inv), -127.), 127.) : 0;
+            w[j >> 2] |= (uint32_t)(n & 255) << (8 * (j & 3));
+        }
+        if (!there) return;
+        *reinterpret_cast<uint2*>(codes + row * D + 8 * c) = uint2{w[0], w[1]};
+        if (c == 0) reinterpret_cast<float*>(scales)[row] = s;
+    } else {
+        top = group_all<4>(top, Max{});
+        const bool whole = group_all<D / 8>(top, Max{}) < kInf;
+        // top = m 2^p, 1 <= m < 2: at most 7 2^e = 1.75 2^(e + 2) with e = p - 2, or p - 1 where m is over 1.75
+        const uint64_t u = __builtin_bit_cast(uint64_t, top);
+        int e = (int)(u >> 52) - 1023 - 2 + ((u & 0xfffffffffffffull) > 0xc000000000000ull);
+        e = min(max(e, -126), 125);
+        const double inv = __builtin_bit_cast(double, (uint64_t)(1023 - e) << 52);
+        uint32_t w = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const double a = fabs(y[j]) * inv;
+            // codes are 1/2 apart up to 2, 1 up to 4, 2 up to 6
+            const double n = rint(a * (a < 2. ? 2. : a < 4. ? 1. : .5));
+            const int code = min((int)fmin(n, 16.) + (a < 2. ? 0 : a < 4. ? 2 : 4), 7);
+            w |= (uint32_t)(code | (y[j] < 0. ? 8 : 0)) << (4 * j);
+        }
+        if (!there) return;
+        *reinterpret_cast<uint32_t*>(codes + row * (D / 2) + 4 * c) = whole ? w : 0;
+        if ((c & 3) == 0) reinterpret_cast<uint8_t*>(scales)[row * (D / 32) + (c >> 2)] = whole ? (uint8_t)(e + 127) : 255;
+    }
+}
+
+struct Place {
+    int64_t row;   // first of page * heads + head rows of the token's slot, head 0; a head further is `page` rows on
+    bool there;
+};
+__device__ __forceinline__ Place place(const Cache& c, const int32_t* bt, int64_t bt_stride, int seqs, int width, int seq, int p) {
+    Place r{0, false};
+    if (p < 0 || seq < 0 || seq >= seqs || p / c.page >= width) return r;
+    const int blk = bt[seq * bt_stride + p / c.page];
+    if (blk < 0 || blk >= c.pages) return r;
+    r.row = (int64_t)blk * c.heads * c.page + p % c.page;
+    r.there = true;
+    return r;
+}
+
+template <int KIND, int D>
+__global__ void __launch_bounds__(256) norm_rope_kv_quant_kernel(
+    const uint16_t* __restrict__ qkv, int64_t qkv_stride, const int32_t* __restrict__ pos, const int32_t* __restrict__ tok_seq,
+    const int32_t* __restrict__ bt, int64_t bt_stride, int seqs, int width, const float* __restrict__ cos_sin, int R, int P,
+    const uint16_t* __restrict__ q_norm, const uint16_t* __restrict__ k_norm, double eps, uint16_t* __restrict__ q_out, Cache cache, int64_t T, int hq) {
+    constexpr int L = D / 8;   // lanes of a head row
+    const int nh = hq + 2 * cache.heads;
+    const int64_t at = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L, unit = at < T * nh ? at : T * nh - 1;
+    const int c = threadIdx.x % L;
+    const int64_t t = unit / nh;
+    const int head = (int)(unit - t * nh);
+    const uint16_t* src = qkv + t * qkv_stride + (int64_t)head * D;
+    float x[8];
+    ld8(src + 8 * c, x);
+    const int p = pos[t];
+    Place pl = place(cache, bt, bt_stride, seqs, width, tok_seq[t], p);
+    pl.there = pl.there && p < P && at == unit;
+    const bool q_row = head < hq;
+    if (head >= hq + cache.heads) {
+        double y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = x[j];
+        put<KIND, D>(y, c, pl.there, cache.v, cache.vs, pl.row + (int64_t)(head - hq - cache.heads) * cache.page);
+        return;
+    }
+    const uint16_t* wn = q_row ? q_norm : k_norm;
+    const int H = R / 16;   // chunks of eight dimensions in a half of the rotation
+    const bool turns = c < 2 * H;
+    const int other = c < H ? c + H : turns ? c - H : c;
+    float xo[8], w[8], wo[8], cs[8], sn[8];
+    ld8(src + 8 * other, xo);
+    double inv = 1.;
+    if (wn) {
+        ld8(wn + 8 * c, w);
+        ld8(wn + 8 * other, wo);
+        double ss = 0.;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss += (double)x[j] * (double)x[j];
+        ss = group_all<L>(ss, Sum{});
+        inv = 1. / sqrt(ss / D + eps);
+    }
+    if (turns) {
+        const float* row = cos_sin + (int64_t)(pl.there ? p : 0) * R + 8 * (c < H ? c : c - H);
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+            *reinterpret_cast<f32x4*>(cs + j) = *reinterpret_cast<const f32x4*>(row + j);
+            *reinterpret_cast<f32x4*>(sn + j) = *reinterpret_cast<const f32x4*>(row + R / 2 + j);
+        }
+    }
+    if (q_row) {
+        const float f = (float)inv;
+        u16x8 o;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float y = x[j], yo = xo[j];
+            if (wn) {
+                y *= f * w[j];
+                yo *= f * wo[j];
+            }
+            if (turns) y = y * cs[j] + yo * (c < H ? -sn[j] : sn[j]);
+            o[j] = pl.there ? f2bf(y) : 0;
+        }
+        if (at == unit) *reinterpret_cast<u16x8*>(q_out + (t * hq + head) * D + 8 * c) = o;
+    } else {
+        double y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            double yo = xo[j];
+            y[j] = x[j];
+            if (wn) {
+                y[j] *= inv * w[j];
+                yo *= inv * wo[j];
+            }
+            if (turns) y[j] = y[j] * cs[j] + yo * (double)(c < H ? -sn[j] : sn[j]);
+        }
+        put<KIND, D>(y, c, pl.there, cache.k, cache.ks, pl.row + (int64_t)(head - hq) * cache.page);
+    }
+}
+
+// k, v [T, Hkv, D] in bfloat16 of tokens of the cache; zeros where a token has no place.  Reads the codes, writes 4 T Hkv D bytes: bytes bound.
+template <int KIND, int D>
+__global__ void __launch_bounds__(256) quant_kv_read_kernel(const int32_t* __restrict__ pos, const int32_t* __restrict__ tok_seq, const int32_t* __restrict__ bt,
+                                                            int64_t bt_stride, int seqs, int width, Cache cache, uint16_t* __restrict__ k,
+                                                            uint16_t* __restrict__ v, int64_t T) {
+    constexpr int L = D / 8;
+    const int64_t unit = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    if (unit >= T * cache.heads) return;
+    const int c = threadIdx.x % L;
+    const int64_t t = unit / cache.heads;
+    const int head = (int)(unit - t * cache.heads);
+    const Place pl = place(cache, bt, bt_stride, seqs, width, tok_seq[t], pos[t]);
+    const int64_t row = pl.row + (int64_t)head * cache.page;
+    auto one = [&](const uint8_t* codes, const void* scales, uint16_t* out) {
+        u16x8 o = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (pl.there) {
+            if constexpr (KIND == kInt8) {
+                const uint2 w = *reinterpret_cast<const uint2*>(codes + row * D + 8 * c);
+                const float s = reinterpret_cast<const float*>(scales)[row];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j] = f2bf(code8(j < 4 ? w.x : w.y, j & 3) * s);
+            } else {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + row * (D / 2) + 4 * c);
+                const uint32_t e = reinterpret_cast<const uint8_t*>(scales)[row * (D / 32) + (c >> 2)];
+                bf16x2 b[4];
+                codes4(w, __uint_as_float(e << 23), b);
+                o = __builtin_bit_cast(u16x8, (bf16x8{b[0][0], b[0][1], b[1][0], b[1][1], b[2][0], b[2][1], b[3][0], b[3][1]}));
+                if (e == 255) o = u16x8{0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0};
+            }
+        }
+        *reinterpret_cast<u16x8*>(out + unit * D + 8 * c) = o;
+    };
+    one(cache.k, cache.ks, k);
+    one(cache.v, cache.vs, v);
+}
+
+}  // namespace
+
+void launch_norm_rope_kv_quant(int kind, int D, const uint16_t* qkv, int64_t qkv_stride, const int32_t* pos, const int32_t* tok_seq, const int32_t* bt,
+                               int64_t bt_stride, int seqs, int width, const float* cos_sin, int R, int P, const uint16_t* q_norm, const uint16_t* k_norm, double eps,
+                               uint16_t* q_out, const Cache& cache, int64_t T, int hq, hipStream_t st) {
+    if (T == 0) return;
+    const int64_t units = T * (hq + 2 * cache.heads), per = 256 / (D / 8);
+    const dim3 g((unsigned)((units + per - 1) / per)), b(256);
+#define CHRONOS_QKV(K, DD)                                                                                                                                    \
+    if (kind == K && D == DD)                                                                                                                                 \
+        hipLaunchKernelGGL((norm_rope_kv_quant_kernel<K, DD>), g, b, 0, st, qkv, qkv_stride, pos, tok_seq, bt, bt_stride, seqs, width, cos_sin, R, P, q_norm, \
+                           k_norm, eps, q_out, cache, T, hq);
+    CHRONOS_QKV(kInt8, 64) CHRONOS_QKV(kInt8, 128) CHRONOS_QKV(kFp4, 64) CHRONOS_QKV(kFp4, 128)
+#undef CHRONOS_QKV
+}
+
+void launch_quant_kv_read(int kind, int D, const int32_t* pos, const int32_t* tok_seq, const int32_t* bt, int64_t bt_stride, int seqs, int width, const Cache& cache,
+                          uint16_t* k, uint16_t* v, int64_t T, hipStream_t st) {
+    if (T == 0) return;
+    const int64_t units = T * cache.heads, per = 256 / (D / 8);
+    const dim3 g((unsigned)((units + per - 1) / per)), b(256);
+#define CHRONOS_QKV(K, DD) \
+    if (kind == K && D == DD) hipLaunchKernelGGL((quant_kv_read_kernel<K, DD>), g, b, 0, st, pos, tok_seq, bt, bt_stride, seqs, width, cache, k, v, T);
+    CHRONOS_QKV(kInt8, 64) CHRONOS_QKV(kInt8, 128) CHRONOS_QKV(kFp4, 64) CHRONOS_QKV(kFp4, 128)
+#undef CHRONOS_QKV
+}
+
+}  // namespace qkv
+}  // namespace chronos

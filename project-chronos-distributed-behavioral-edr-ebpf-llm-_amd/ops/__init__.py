@@ -310,3 +310,7 @@ def pick_nsplit(n_workgroups: int, max_ctx: int, cus: int = 256) -> int:
     want = (_SPLIT_WGS * cus + n_workgroups - 1) // n_workgroups
     cap = max(1, max_ctx // 256)
     return int(max(1, min(want, cap, _SPLIT_MAX)))
+
+
+from .quant_kv import (QuantKV, norm_rope_kv_quant, prefix_attention, quant_attention, quant_kv_cache,  # noqa: E402,F401
+                       quant_kv_read)
