@@ -460,44 +460,61 @@ __global__ void __launch_bounds__(256, NQT <= 2 ? 2 : 1) quant_rows_kernel(const
     }
 }
 
-// Rows of the pieces' sums: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  `per` groups of D / 4 lanes share a row's pieces and are joined through LDS.
+// Rows of the pieces' sums: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  D / 4 lanes have a row, `per` such groups share its pieces and are joined through
+// LDS.  The maxima and sums of up to D / 4 pieces are read at once, a lane each, and handed round; what the pieces hold does not wait for them.
 template <int D>
 __global__ void __launch_bounds__(256) quant_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, uint16_t* __restrict__ out, int64_t rows,
                                                          int slots, int per) {
     constexpr int L = D / 4, GR = 256 / L;
     __shared__ f32x4 so[GR][L];
-    __shared__ float sl[GR];
+    __shared__ float sl[GR], sm[GR];
     const int c = threadIdx.x % L, gr = threadIdx.x / L;
-    const int64_t row = (int64_t)blockIdx.x * (GR / per) + gr / per;
-    const bool live = row < rows;
-    float mx = -INFINITY;
-    if (live)
-        for (int s = 0; s < slots; ++s) {
-            const float2 ml = part_ml[s * rows + row];
-            if (ml.y != 0.f) mx = fmaxf(mx, ml.x);
-        }
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float l = 0.f;
+    const int64_t at = (int64_t)blockIdx.x * (GR / per) + gr / per, row = at < rows ? at : rows - 1;
+    float mx = -INFINITY, l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    if (live)
-        for (int s = gr % per; s < slots; s += per) {
-            const float2 ml = part_ml[s * rows + row];
-            if (ml.y == 0.f) continue;
-            const float f = __builtin_amdgcn_exp2f(ml.x - base);
-            l += ml.y * f;
-            o += *reinterpret_cast<const f32x4*>(part_o + (s * rows + row) * D + 4 * c) * f;
-        }
-    if (per > 1) {
-        so[gr][c] = o;
-        if (c == 0) sl[gr] = l;
-        __syncthreads();
-        if (gr % per) return;
-        for (int i = 1; i < per; ++i) {
-            o += so[gr + i][c];
-            l += sl[gr + i];
+    for (int s0 = gr % per; s0 < slots; s0 += per * L) {   // pieces s0, s0 + per, ..: lane c has the c-th
+        const int n = min(L, (slots - s0 + per - 1) / per), mine = s0 + per * c;
+        const float2 ml = c < n ? part_ml[mine * rows + row] : float2{-INFINITY, 0.f};
+        const bool there = ml.y != 0.f;
+        float top = there ? ml.x : -INFINITY;
+#pragma unroll
+        for (int k = 1; k < L; k <<= 1) top = fmaxf(top, __shfl_xor(top, k, L));
+        top = fmaxf(top, mx);
+        const float base = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(mx - base);
+        mx = top;
+        l *= old;
+        o *= old;
+        const float w = there ? __builtin_amdgcn_exp2f(ml.x - base) : 0.f;
+        float sum = there ? ml.y * w : 0.f;
+#pragma unroll
+        for (int k = 1; k < L; k <<= 1) sum += __shfl_xor(sum, k, L);
+        l += sum;
+        const float* p = part_o + (s0 * rows + row) * D + 4 * c;
+#pragma unroll 4
+        for (int i = 0; i < n; ++i, p += per * rows * D) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(p);
+            const float f = __shfl(w, i, L);
+            const bool on = __shfl((int)there, i, L);   // what an empty piece has there was never written
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] += on ? x[j] * f : 0.f;
         }
     }
-    if (!live) return;
+    if (per > 1) {
+        so[gr][c] = o;
+        if (c == 0) sl[gr] = l, sm[gr] = mx;
+        __syncthreads();
+        if (gr % per) return;
+        for (int i = 1; i < per; ++i) mx = fmaxf(mx, sm[gr + i]);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        l = 0.f;
+        o = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < per; ++i) {
+            const float f = __builtin_amdgcn_exp2f(sm[gr + i] - base);
+            o += so[gr + i][c] * f;
+            l += sl[gr + i] * f;
+        }
+    }
+    if (at >= rows) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     *reinterpret_cast<u16x4*>(out + row * D + 4 * c) = u16x4{f2bf(o[0] * inv), f2bf(o[1] * inv), f2bf(o[2] * inv), f2bf(o[3] * inv)};
 }

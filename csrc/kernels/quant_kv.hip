@@ -7,7 +7,8 @@
 // It reads T (Hq + 2 Hkv) D 2 bytes and writes T Hq D 2 and the rows' codes: bytes are what bounds it.  D / 8 lanes a head row, 16 bytes a lane; a lane's rotation
 // partner is D / 16 lanes away or none, and its eight numbers are read a second time (they are in the cache) where an exchange would go through LDS.  Keys and values
 // go by double up to their codes: a key next to a border between two codes then takes the code of the formula, whatever the order of sums, and it costs nothing
-// beside the bytes.  Queries are float32 but for their sum of squares.
+// beside the bytes (the queries,
+// most of the rows, are float32: all rows in double took 237 us for 16384 tokens of 64 + 16 heads, against PLACE).
 #include "chronos_quant_kv.h"
 
 namespace chronos {
@@ -51,7 +52,7 @@ template <int KIND, int D> __device__ __forceinline__ void put(const double (&y)
         uint32_t w[2] = {0, 0};
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int n = inv > 0. ? (int)fmin(fmax(rint(y[j] * inv), -127.), 127.) : 0;
+            const int n = whole ? min(max((int)rint(y[j] * inv), -127), 127) : 0;   // past 127 where the scale is denormal
             w[j >> 2] |= (uint32_t)(n & 255) << (8 * (j & 3));
         }
         if (!there) return;
@@ -94,119 +95,162 @@ __device__ __forceinline__ Place place(const Cache& c, const int32_t* bt, int64_
     return r;
 }
 
-template <int KIND, int D>
+// A block has 256 / (D / 8) * N neighbouring query heads of a token (the place, the angles and the weights serve all of them, the rows' loads are under way together),
+// or 256 / (D / 8) of its key and value heads: `parts` blocks a token, the first q_parts with queries.
+template <int KIND, int D, int N>
 __global__ void __launch_bounds__(256) norm_rope_kv_quant_kernel(
     const uint16_t* __restrict__ qkv, int64_t qkv_stride, const int32_t* __restrict__ pos, const int32_t* __restrict__ tok_seq,
     const int32_t* __restrict__ bt, int64_t bt_stride, int seqs, int width, const float* __restrict__ cos_sin, int R, int P,
-    const uint16_t* __restrict__ q_norm, const uint16_t* __restrict__ k_norm, double eps, uint16_t* __restrict__ q_out, Cache cache, int64_t T, int hq) {
-    constexpr int L = D / 8;   // lanes of a head row
-    const int nh = hq + 2 * cache.heads;
-    const int64_t at = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L, unit = at < T * nh ? at : T * nh - 1;
-    const int c = threadIdx.x % L;
-    const int64_t t = unit / nh;
-    const int head = (int)(unit - t * nh);
-    const uint16_t* src = qkv + t * qkv_stride + (int64_t)head * D;
-    float x[8];
-    ld8(src + 8 * c, x);
-    const int p = pos[t];
-    Place pl = place(cache, bt, bt_stride, seqs, width, tok_seq[t], p);
-    pl.there = pl.there && p < P && at == unit;
-    const bool q_row = head < hq;
-    if (head >= hq + cache.heads) {
-        double y[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = x[j];
-        put<KIND, D>(y, c, pl.there, cache.v, cache.vs, pl.row + (int64_t)(head - hq - cache.heads) * cache.page);
-        return;
-    }
-    const uint16_t* wn = q_row ? q_norm : k_norm;
+    const uint16_t* __restrict__ q_norm, const uint16_t* __restrict__ k_norm, double eps, uint16_t* __restrict__ q_out, Cache cache, int hq, int q_parts, int parts) {
+    constexpr int L = D / 8, S = 256 / L;   // lanes of a head row, head rows side by side
+    const int64_t t = blockIdx.x / parts;
+    const int part = blockIdx.x % parts, c = threadIdx.x % L;
     const int H = R / 16;   // chunks of eight dimensions in a half of the rotation
     const bool turns = c < 2 * H;
-    const int other = c < H ? c + H : turns ? c - H : c;
-    float xo[8], w[8], wo[8], cs[8], sn[8];
-    ld8(src + 8 * other, xo);
-    double inv = 1.;
-    if (wn) {
-        ld8(wn + 8 * c, w);
-        ld8(wn + 8 * other, wo);
-        double ss = 0.;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ss += (double)x[j] * (double)x[j];
-        ss = group_all<L>(ss, Sum{});
-        inv = 1. / sqrt(ss / D + eps);
-    }
-    if (turns) {
-        const float* row = cos_sin + (int64_t)(pl.there ? p : 0) * R + 8 * (c < H ? c : c - H);
-#pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-            *reinterpret_cast<f32x4*>(cs + j) = *reinterpret_cast<const f32x4*>(row + j);
-            *reinterpret_cast<f32x4*>(sn + j) = *reinterpret_cast<const f32x4*>(row + R / 2 + j);
-        }
-    }
-    if (q_row) {
-        const float f = (float)inv;
-        u16x8 o;
+    const int other = c < H ? c + H : turns ? c - H : c;   // the lane's partner's; its numbers count for nothing where there is none
+    const uint16_t* src = qkv + t * qkv_stride;
+    const int p = pos[t], seq = tok_seq[t];
+    const u16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+    float cs[8], sn[8];
+    auto angles = [&](bool there) {
+        const float* row = cos_sin + (int64_t)(there ? p : 0) * R + 8 * (c < H ? c : turns ? c - H : 0);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            float y = x[j], yo = xo[j];
-            if (wn) {
-                y *= f * w[j];
-                yo *= f * wo[j];
-            }
-            if (turns) y = y * cs[j] + yo * (c < H ? -sn[j] : sn[j]);
-            o[j] = pl.there ? f2bf(y) : 0;
+            cs[j] = row[j];
+            sn[j] = row[R / 2 + j];
         }
-        if (at == unit) *reinterpret_cast<u16x8*>(q_out + (t * hq + head) * D + 8 * c) = o;
-    } else {
-        double y[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            double yo = xo[j];
-            y[j] = x[j];
-            if (wn) {
-                y[j] *= inv * w[j];
-                yo *= inv * wo[j];
-            }
-            if (turns) y[j] = y[j] * cs[j] + yo * (double)(c < H ? -sn[j] : sn[j]);
+            cs[j] = turns ? cs[j] : 1.f;
+            sn[j] = c < H ? -sn[j] : sn[j];
         }
-        put<KIND, D>(y, c, pl.there, cache.k, cache.ks, pl.row + (int64_t)(head - hq) * cache.page);
+    };
+    // a row's numbers are inv * (x cs w + x' sn w'), x' and w' the partner's
+    if (part < q_parts) {
+        const int head0 = part * (S * N) + threadIdx.x / L;
+        u16x8 xr[N], xp[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint16_t* row = src + (int64_t)min(head0 + S * i, hq - 1) * D;
+            xr[i] = *reinterpret_cast<const u16x8*>(row + 8 * c);
+            xp[i] = *reinterpret_cast<const u16x8*>(row + 8 * other);
+        }
+        float w[8], wo[8];
+        if (q_norm) {
+            ld8(q_norm + 8 * c, w);
+            ld8(q_norm + 8 * other, wo);
+        }
+        const bool there = place(cache, bt, bt_stride, seqs, width, seq, p).there && p < P;
+        angles(there);
+        if (q_norm) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) cs[j] *= w[j], sn[j] *= wo[j];
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const u16x8 po = turns ? xp[i] : zero;
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = bf2f(xr[i][j]);
+            float f = 1.f;
+            if (q_norm) {
+                float ss = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
+                f = rsqrtf(group_sum(ss, L) * (1.f / D) + (float)eps);
+            }
+            u16x8 o;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = f2bf(f * (x[j] * cs[j] + bf2f(po[j]) * sn[j]));
+            if (head0 + S * i < hq) *reinterpret_cast<u16x8*>(q_out + (t * hq + head0 + S * i) * D + 8 * c) = there ? o : zero;
+        }
+        return;
     }
+    const int at = (part - q_parts) * S + threadIdx.x / L, head = min(at, 2 * cache.heads - 1);
+    const uint16_t* row = src + (int64_t)(hq + head) * D;
+    const bool key = head < cache.heads;
+    const u16x8 xr = *reinterpret_cast<const u16x8*>(row + 8 * c), xp = *reinterpret_cast<const u16x8*>(row + 8 * other);
+    Place pl = place(cache, bt, bt_stride, seqs, width, seq, p);
+    pl.there = pl.there && p < P;
+    double y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = bf2f(xr[j]);
+    if (key) {
+        const u16x8 po = turns ? xp : zero;
+        angles(pl.there);
+        double inv = 1.;
+        float w[8], wo[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = 1.f, wo[j] = 1.f;
+        if (k_norm) {
+            ld8(k_norm + 8 * c, w);
+            ld8(k_norm + 8 * other, wo);
+            double ss = 0.;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ss += y[j] * y[j];
+            inv = 1. / sqrt(group_all<L>(ss, Sum{}) * (1. / D) + eps);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = inv * (y[j] * cs[j] * w[j] + (double)bf2f(po[j]) * sn[j] * wo[j]);
+    }
+    pl.row += (int64_t)(key ? head : head - cache.heads) * cache.page;
+    put<KIND, D>(y, c, pl.there && at == head, key ? cache.k : cache.v, key ? cache.ks : cache.vs, pl.row);
 }
 
-// k, v [T, Hkv, D] in bfloat16 of tokens of the cache; zeros where a token has no place.  Reads the codes, writes 4 T Hkv D bytes: bytes bound.
-template <int KIND, int D>
+// k, v [T, Hkv, D] in bfloat16 of tokens of the cache; zeros where a token has no place.  Reads the codes, writes 4 T Hkv D bytes: bytes bound.  N head rows a lane,
+// their places, then their codes under way together.
+template <int KIND, int D, int N>
 __global__ void __launch_bounds__(256) quant_kv_read_kernel(const int32_t* __restrict__ pos, const int32_t* __restrict__ tok_seq, const int32_t* __restrict__ bt,
                                                             int64_t bt_stride, int seqs, int width, Cache cache, uint16_t* __restrict__ k,
                                                             uint16_t* __restrict__ v, int64_t T) {
-    constexpr int L = D / 8;
-    const int64_t unit = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-    if (unit >= T * cache.heads) return;
+    constexpr int L = D / 8, S = 256 / L, W = KIND == kInt8 ? 2 : 1;
     const int c = threadIdx.x % L;
-    const int64_t t = unit / cache.heads;
-    const int head = (int)(unit - t * cache.heads);
-    const Place pl = place(cache, bt, bt_stride, seqs, width, tok_seq[t], pos[t]);
-    const int64_t row = pl.row + (int64_t)head * cache.page;
-    auto one = [&](const uint8_t* codes, const void* scales, uint16_t* out) {
-        u16x8 o = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (pl.there) {
-            if constexpr (KIND == kInt8) {
-                const uint2 w = *reinterpret_cast<const uint2*>(codes + row * D + 8 * c);
-                const float s = reinterpret_cast<const float*>(scales)[row];
+    const int64_t first = (int64_t)blockIdx.x * (S * N) + threadIdx.x / L, most = T * cache.heads;
+    int64_t row[N];
+    bool there[N];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = f2bf(code8(j < 4 ? w.x : w.y, j & 3) * s);
+    for (int i = 0; i < N; ++i) {
+        const int64_t at = first + S * i, unit = at < most ? at : most - 1, t = unit / cache.heads;
+        const Place pl = place(cache, bt, bt_stride, seqs, width, tok_seq[t], pos[t]);
+        there[i] = pl.there;
+        row[i] = pl.row + (unit - t * cache.heads) * cache.page;   // a row of the cache in any case
+    }
+    uint32_t w[2][N][W], e[2][N];
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+        const uint8_t* codes = kv ? cache.v : cache.k;
+        const void* scales = kv ? cache.vs : cache.ks;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (KIND == kInt8) {
+                const uint2 x = *reinterpret_cast<const uint2*>(codes + row[i] * D + 8 * c);
+                w[kv][i][0] = x.x, w[kv][i][1] = x.y;
+                e[kv][i] = reinterpret_cast<const uint32_t*>(scales)[row[i]];
             } else {
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + row * (D / 2) + 4 * c);
-                const uint32_t e = reinterpret_cast<const uint8_t*>(scales)[row * (D / 32) + (c >> 2)];
-                bf16x2 b[4];
-                codes4(w, __uint_as_float(e << 23), b);
-                o = __builtin_bit_cast(u16x8, (bf16x8{b[0][0], b[0][1], b[1][0], b[1][1], b[2][0], b[2][1], b[3][0], b[3][1]}));
-                if (e == 255) o = u16x8{0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0};
+                w[kv][i][0] = *reinterpret_cast<const uint32_t*>(codes + row[i] * (D / 2) + 4 * c);
+                e[kv][i] = reinterpret_cast<const uint8_t*>(scales)[row[i] * (D / 32) + (c >> 2)];
             }
         }
-        *reinterpret_cast<u16x8*>(out + unit * D + 8 * c) = o;
-    };
-    one(cache.k, cache.ks, k);
-    one(cache.v, cache.vs, v);
+    }
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (first + S * i >= most) break;
+            u16x8 o;
+            if constexpr (KIND == kInt8) {
+                const float s = __uint_as_float(e[kv][i]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j] = f2bf(code8(w[kv][i][j >> 2], j & 3) * s);
+            } else {
+                bf16x2 b[4];
+                codes4(w[kv][i][0], __uint_as_float(e[kv][i] << 23), b);
+                o = __builtin_bit_cast(u16x8, (bf16x8{b[0][0], b[0][1], b[1][0], b[1][1], b[2][0], b[2][1], b[3][0], b[3][1]}));
+                if (e[kv][i] == 255) o = u16x8{0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0};
+            }
+            if (!there[i]) o = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+            *reinterpret_cast<u16x8*>((kv ? v : k) + (first + S * i) * D + 8 * c) = o;
+        }
 }
 
 }  // namespace
@@ -215,24 +259,31 @@ void launch_norm_rope_kv_quant(int kind, int D, const uint16_t* qkv, int64_t qkv
                                int64_t bt_stride, int seqs, int width, const float* cos_sin, int R, int P, const uint16_t* q_norm, const uint16_t* k_norm, double eps,
                                uint16_t* q_out, const Cache& cache, int64_t T, int hq, hipStream_t st) {
     if (T == 0) return;
-    const int64_t units = T * (hq + 2 * cache.heads), per = 256 / (D / 8);
-    const dim3 g((unsigned)((units + per - 1) / per)), b(256);
-#define CHRONOS_QKV(K, DD)                                                                                                                                    \
-    if (kind == K && D == DD)                                                                                                                                 \
-        hipLaunchKernelGGL((norm_rope_kv_quant_kernel<K, DD>), g, b, 0, st, qkv, qkv_stride, pos, tok_seq, bt, bt_stride, seqs, width, cos_sin, R, P, q_norm, \
-                           k_norm, eps, q_out, cache, T, hq);
-    CHRONOS_QKV(kInt8, 64) CHRONOS_QKV(kInt8, 128) CHRONOS_QKV(kFp4, 64) CHRONOS_QKV(kFp4, 128)
+    const int side = 256 / (D / 8);
+    // four head rows a lane where the card is full all the same
+    const bool four = T * ((hq + 4 * side - 1) / (4 * side)) >= 1024;
+    const int q_parts = (hq + (four ? 4 : 1) * side - 1) / ((four ? 4 : 1) * side), parts = q_parts + (2 * cache.heads + side - 1) / side;
+    const dim3 g((unsigned)(T * parts)), b(256);
+#define CHRONOS_QKV(K, DD, N)                                                                                                                                        \
+    if (kind == K && D == DD && four == (N == 4))                                                                                                                    \
+        hipLaunchKernelGGL((norm_rope_kv_quant_kernel<K, DD, N>), g, b, 0, st, qkv, qkv_stride, pos, tok_seq, bt, bt_stride, seqs, width, cos_sin, R, P, q_norm,     \
+                           k_norm, eps, q_out, cache, hq, q_parts, parts);
+    CHRONOS_QKV(kInt8, 64, 1) CHRONOS_QKV(kInt8, 128, 1) CHRONOS_QKV(kFp4, 64, 1) CHRONOS_QKV(kFp4, 128, 1)
+    CHRONOS_QKV(kInt8, 64, 4) CHRONOS_QKV(kInt8, 128, 4) CHRONOS_QKV(kFp4, 64, 4) CHRONOS_QKV(kFp4, 128, 4)
 #undef CHRONOS_QKV
 }
 
 void launch_quant_kv_read(int kind, int D, const int32_t* pos, const int32_t* tok_seq, const int32_t* bt, int64_t bt_stride, int seqs, int width, const Cache& cache,
                           uint16_t* k, uint16_t* v, int64_t T, hipStream_t st) {
     if (T == 0) return;
-    const int64_t units = T * cache.heads, per = 256 / (D / 8);
-    const dim3 g((unsigned)((units + per - 1) / per)), b(256);
-#define CHRONOS_QKV(K, DD) \
-    if (kind == K && D == DD) hipLaunchKernelGGL((quant_kv_read_kernel<K, DD>), g, b, 0, st, pos, tok_seq, bt, bt_stride, seqs, width, cache, k, v, T);
-    CHRONOS_QKV(kInt8, 64) CHRONOS_QKV(kInt8, 128) CHRONOS_QKV(kFp4, 64) CHRONOS_QKV(kFp4, 128)
+    const int64_t units = T * cache.heads, side = 256 / (D / 8);
+    const bool four = units >= 4 * side * 1024;
+    const dim3 g((unsigned)((units + (four ? 4 : 1) * side - 1) / ((four ? 4 : 1) * side))), b(256);
+#define CHRONOS_QKV(K, DD, N)                    \
+    if (kind == K && D == DD && four == (N == 4)) \
+        hipLaunchKernelGGL((quant_kv_read_kernel<K, DD, N>), g, b, 0, st, pos, tok_seq, bt, bt_stride, seqs, width, cache, k, v, T);
+    CHRONOS_QKV(kInt8, 64, 1) CHRONOS_QKV(kInt8, 128, 1) CHRONOS_QKV(kFp4, 64, 1) CHRONOS_QKV(kFp4, 128, 1)
+    CHRONOS_QKV(kInt8, 64, 4) CHRONOS_QKV(kInt8, 128, 4) CHRONOS_QKV(kFp4, 64, 4) CHRONOS_QKV(kFp4, 128, 4)
 #undef CHRONOS_QKV
 }
 
