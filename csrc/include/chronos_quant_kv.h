@@ -22,10 +22,10 @@ struct Cache {
     int pages, heads, page;
 };
 
-// How a call of the attention is cut up (quant_attention.hip): rows of a tile in 16s, tiles and pieces of the keys, for the sequences' own keys and for those that
+// How a call of the attention is cut up (quant_attention.hip): rows of a tile, tiles and pieces of the keys, for the sequences' own keys and for those that
 // groups share; slots of partial sums, 1: none
 struct AttnPlan {
-    int own_nqt, own_splits, group_nqt, group_splits, slots;
+    int own_rows, own_splits, group_rows, group_splits, slots;
     int64_t own_tiles, group_tiles;
 };
 

@@ -10,12 +10,16 @@
 //   * K: the dimensions of a product may be taken in any order that queries and keys share, so a lane takes its row's bytes 16 at a time;
 //   * V: the operand wants eight keys of one dimension, the page has the dimensions of one key.  Row m of product dt is dimension m D / 16 + dt: a lane then needs the
 //     same D / 16 neighbouring bytes of its eight keys, for all products, and no exchange between lanes.
-// int8: a key's scale multiplies its scores, a value's the probabilities, in float32 before they are rounded to bfloat16 (2^-9, as everywhere in this library:
-// rows average many of them and the output has the same step).  mxfp4: the conversion takes the scale.
+// int8: a key's scale multiplies its scores, a value's the probabilities.  These are then rounded to float16 (2^-12): in bfloat16 the largest probability of a row, 1 times a scale, would
+// be off by up to 2^-9 where without scales it is exact (.0025 of the output's size in place of .0017, of which its own rounding is .0016).  float16 has the range as they are held as a part of the largest
+// scale so far: down to 2^-38 of it.  mxfp4: the conversion takes the scale, probabilities are bfloat16.
 //
 // What no sum may take: keys behind the position, behind the context, on pages that the table does not have (numbers outside 0 .. pages - 1 are left out): their
 // scores are -inf and their probabilities zero by selection, not by product; their values cannot be NaN either (a value scale of NaN acts on the probabilities of
 // rows that see it).  Rows without any key are zeros.
+#include <limits.h>
+
+#include "chronos_lds.h"
 #include "chronos_quant_kv.h"
 
 namespace chronos {
@@ -38,6 +42,7 @@ struct AttnArgs {
     float* part_o;            // [slots, T * hq, D]
     float2* part_ml;          // [slots, T * hq]: maximum (base 2) and sum
     int slots, splits, slot0;
+    int page_shift;           // pages of a power of two tokens; -1: others
 };
 
 namespace {
@@ -107,29 +112,93 @@ __device__ __forceinline__ int shared_of(const AttnArgs& a, int seq, int lane) {
     return g >= 0 && g < a.groups ? shared_keys(a, g) : -1;
 }
 
+// What a workgroup's item is: its sequence (of a group: the one whose table is read), context and the keys that the launch has of it
+template <bool GROUPS> struct Item {
+    int seq, ctx, k0;
+    __device__ __forceinline__ Item(const AttnArgs& a, const Tile& t, int lane) : seq(t.item), ctx(0), k0(0) {
+        if constexpr (GROUPS) {
+            seq = min(first_seq(a, t.item), a.B - 1);
+        } else {
+            if (seq < a.B) {
+                ctx = (int)min((int64_t)max(a.ctx_len[seq], 0), (int64_t)a.width * a.cache.page);
+                if (a.group_start) k0 = shared_of(a, seq, lane);
+            } else {
+                k0 = -1;
+                seq = 0;
+            }
+        }
+    }
+    // the last position that token t sees
+    __device__ __forceinline__ int sees(const AttnArgs& a, const Tile& tile, int t) const {
+        if constexpr (!GROUPS) return ctx - tile.toks + (t - tile.tok0);
+        int s0 = first_seq(a, tile.item), s1 = first_seq(a, tile.item + 1) - 1;   // the token's sequence: the last that begins at or before it
+        if (a.q_start) {
+            while (s0 < s1) {
+                const int mid = (s0 + s1 + 1) >> 1;
+                if (first_row(a, mid) <= t) s0 = mid;
+                else s1 = mid - 1;
+            }
+        } else {
+            s0 = t;
+        }
+        return min(a.ctx_len[s0], a.width * a.cache.page) - first_row(a, s0 + 1) + t;
+    }
+    // keys [k0, the end) of rows that see up to `last`; a piece of them
+    __device__ __forceinline__ void piece(const AttnArgs& a, const Tile& tile, int last, int split, int unit, int& from, int& to) const {
+        int k1;
+        if constexpr (GROUPS) k1 = min(shared_keys(a, tile.item), last + 1);
+        else k1 = min(ctx, last + 1);
+        const int b = max(k0, 0), n = max(k1 - b, 0);
+        const int chunk = max(((n + a.splits - 1) / a.splits + unit - 1) / unit * unit, unit);
+        from = (int)min((int64_t)b + (int64_t)split * chunk, (int64_t)INT_MAX - 1024);
+        to = min(k1, from + chunk);
+    }
+    // rows of a sequence outside all groups: nothing is written to the slots of what groups share, so the first piece marks them empty
+    __device__ __forceinline__ void mark(const AttnArgs& a, const Tile& tile, int rows, int h, int G, int threads) const {
+        if constexpr (!GROUPS)
+            if (k0 < 0 && a.slot0 > 0)
+                for (int i = threadIdx.x; i < rows * a.slot0; i += threads) {
+                    const int R = tile.at + i % rows;
+                    if (R < tile.toks * G)
+                        a.part_ml[(int64_t)(i / rows) * a.T * a.hq + (int64_t)(tile.tok0 + R / G) * a.hq + h * G + R % G] = float2{-INFINITY, 0.f};
+                }
+    }
+};
+
 // ---- codes to operands --------------------------------------------------------------------------------------------------------------------------------
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
 template <int KIND, int D> struct Step {   // 32 keys of one wave
     static constexpr int KW = row_bytes<KIND, D>() / 16;   // words of K a lane has of a key: a quarter of the row
     static constexpr int VW = row_bytes<KIND, D>() >= 64 ? row_bytes<KIND, D>() / 64 : 1;   // words of V a lane has of a key: a sixteenth of the row
     uint32_t k[2][KW], v[8][VW];
     f32x4 ks[2], vs[2];      // int8: scales of keys 16 g + 4 h4 + i
     uint32_t ke[2], ve[8];   // mxfp4: E of the lane's key and block; words of all blocks' E of its eight keys
-    bool ok[2];              // the page is there
+};
+struct Pages {   // of a step's two halves; -1: not there
+    int blk[2], off[2];
 };
 
-template <int KIND, int D> __device__ __forceinline__ void load_step(const AttnArgs& a, const int32_t* bt, int h, int t0, int end, int lane, Step<KIND, D>& s) {
+__device__ __forceinline__ Pages find_pages(const AttnArgs& a, const int32_t* bt, int t0, int end) {
+    Pages p;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        const int at = t0 + 16 * g;
+        const int i = a.page_shift >= 0 ? at >> a.page_shift : at / a.cache.page;
+        const int blk = at < end ? __builtin_amdgcn_readfirstlane(bt[i]) : -1;
+        p.blk[g] = blk < a.cache.pages ? blk : -1;
+        p.off[g] = at - i * a.cache.page;
+    }
+    return p;
+}
+
+template <int KIND, int D> __device__ __forceinline__ void load_step(const AttnArgs& a, const Pages& p, int h, int lane, Step<KIND, D>& s) {
     constexpr int RB = row_bytes<KIND, D>();
-    using S = Step<KIND, D>;
     const int r = lane & 15, h4 = lane >> 4;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-        const int tg = t0 + 16 * g;
-        const bool in = tg < end;
-        const int at = in ? tg : t0;
-        int blk = __builtin_amdgcn_readfirstlane(bt[at / a.cache.page]);
-        s.ok[g] = in && blk >= 0 && blk < a.cache.pages;
-        if (!s.ok[g]) blk = 0;
-        const int64_t row = ((int64_t)blk * a.cache.heads + h) * a.cache.page + at % a.cache.page;   // of 16, all of one page
+        const int64_t row = ((int64_t)max(p.blk[g], 0) * a.cache.heads + h) * a.cache.page + p.off[g];   // of 16, all of one page
         const uint8_t* kp = a.cache.k + (row + r) * RB;
         if constexpr (KIND == kInt8) {
 #pragma unroll
@@ -147,18 +216,14 @@ template <int KIND, int D> __device__ __forceinline__ void load_step(const AttnA
                 const uint2 x = *reinterpret_cast<const uint2*>(kp + 8 * h4);
                 s.k[g][0] = x.x, s.k[g][1] = x.y;
             }
-            const uint8_t* ke = reinterpret_cast<const uint8_t*>(a.cache.ks) + (row + r) * (D / 32) + h4 * (D / 32) / 4;
-            s.ke[g] = *ke;
+            s.ke[g] = *(reinterpret_cast<const uint8_t*>(a.cache.ks) + (row + r) * (D / 32) + h4 * (D / 32) / 4);
             const uint8_t* ve = reinterpret_cast<const uint8_t*>(a.cache.vs) + (row + 4 * h4) * (D / 32);
             if constexpr (D == 128) {
                 const uint4 x = *reinterpret_cast<const uint4*>(ve);
                 s.ve[4 * g] = x.x, s.ve[4 * g + 1] = x.y, s.ve[4 * g + 2] = x.z, s.ve[4 * g + 3] = x.w;
             } else {
                 const uint2 w = *reinterpret_cast<const uint2*>(ve);
-                s.ve[4 * g] = w.x & 0xffff;
-                s.ve[4 * g + 1] = w.x >> 16;
-                s.ve[4 * g + 2] = w.y & 0xffff;
-                s.ve[4 * g + 3] = w.y >> 16;
+                s.ve[4 * g] = w.x & 0xffff, s.ve[4 * g + 1] = w.x >> 16, s.ve[4 * g + 2] = w.y & 0xffff, s.ve[4 * g + 3] = w.y >> 16;
             }
         }
 #pragma unroll
@@ -196,30 +261,55 @@ template <int KIND, int D> __device__ __forceinline__ bf16x8 key_operand(const S
         return bf16x8{b[0][0], b[0][1], b[1][0], b[1][1], b[2][0], b[2][1], b[3][0], b[3][1]};
     }
 }
-// V operands of all products: dimension r D / 16 + dt, keys 4 h4 .. + 3 and 16 + 4 h4 .. + 3
-template <int KIND, int D> __device__ __forceinline__ void value_operands(const Step<KIND, D>& s, int r, bf16x8 (&o)[D / 16]) {
-    if constexpr (KIND == kInt8) {
+// V operands: dimension r D / 16 + dt, keys 4 h4 .. + 3 and 16 + 4 h4 .. + 3.
+// int8: float16 of the code / 512, two keys at a time: the byte, its top bit turned, is a denormal float16 of u 2^-24, u = code + 128; one fused multiply-add (with 2^15 and -1/4) makes
+// code / 512 of it, exactly.
+constexpr float kCodeUnit = 1.f / 512.f;
+__device__ __forceinline__ uint32_t pair8(uint32_t first, uint32_t second, int i) {   // words with their top bits turned; byte i of both
+    const uint32_t u = __builtin_amdgcn_perm(second, first, 0x0c040c00u + 0x00010001u * (uint32_t)i);
+    const f16x2 x = __builtin_bit_cast(f16x2, u);
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x, f16x2{(_Float16)32768.f, (_Float16)32768.f}, f16x2{(_Float16)-0.25f, (_Float16)-0.25f}));
+}
+template <int KIND, int D> struct Values {
+    uint32_t w[D / 16][4];   // operand dt: eight 16-bit numbers
+    __device__ __forceinline__ void make(Step<KIND, D>& s, int r) {
+        if constexpr (KIND == kInt8) {
 #pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt)
+            for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o[dt][j] = (__bf16)code8(s.v[j][dt >> 2], dt & 3);
-    } else {
-        const int sh = 8 * (r * (D / 16) / 32);
+                for (int x = 0; x < Step<KIND, D>::VW; ++x) s.v[j][x] ^= 0x80808080u;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float scale = __uint_as_float(((s.ve[j] >> sh) & 255) << 23);
-            bf16x2 b[4];
-            codes4(s.v[j][0], scale, b);
+            for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
-            for (int dt = 0; dt < D / 16; ++dt) o[dt][j] = b[dt >> 1][dt & 1];
+                for (int j = 0; j < 4; ++j) w[dt][j] = pair8(s.v[2 * j][dt >> 2], s.v[2 * j + 1][dt >> 2], dt & 3);
+        } else {
+            const int sh = 8 * (r * (D / 16) / 32);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                bf16x2 a[4], b[4];
+                codes4(s.v[2 * j][0], __uint_as_float(((s.ve[2 * j] >> sh) & 255) << 23), a);
+                codes4(s.v[2 * j + 1][0], __uint_as_float(((s.ve[2 * j + 1] >> sh) & 255) << 23), b);
+#pragma unroll
+                for (int dt = 0; dt < D / 16; ++dt)
+                    w[dt][j] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b[dt >> 1]), __builtin_bit_cast(uint32_t, a[dt >> 1]), dt & 1 ? 0x07060302u : 0x05040100u);
+            }
         }
     }
+    __device__ __forceinline__ f32x4 mul(int dt, const uint32_t (&p)[4], f32x4 acc) const {
+        const uint4 x{w[dt][0], w[dt][1], w[dt][2], w[dt][3]}, y{p[0], p[1], p[2], p[3]};
+        if constexpr (KIND == kInt8) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), acc, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), acc, 0, 0, 0);
+    }
+};
+template <int KIND> __device__ __forceinline__ uint32_t round2(float a, float b) {
+    if constexpr (KIND == kInt8) return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+    else return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
 }
 
 // ---- the tile -----------------------------------------------------------------------------------------------------------------------------------------
 // GROUPS: the items are groups of sequences, the keys those that each shares; otherwise sequences, their keys behind what they share.
 template <int KIND, int D, int NQT, bool GROUPS>
-__global__ void __launch_bounds__(256, NQT <= 2 ? 2 : 1) quant_rows_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_rows_kernel(const AttnArgs a) {
     constexpr int ROWS = 16 * NQT, NC = D / 32, ND = D / 16;
     __shared__ __attribute__((aligned(16))) f32x4 so[3][ND][64];
     __shared__ float sm[3][64], sl[3][64];
@@ -231,49 +321,17 @@ __global__ void __launch_bounds__(256, NQT <= 2 ? 2 : 1) quant_rows_kernel(const
     if (!find_tile<GROUPS>(a, blockIdx.x / heads, G, ROWS, lane, tile)) return;
 
     // the rows of this lane: the last position each sees, and its queries
+    const Item<GROUPS> item(a, tile, lane);
+    if (split == 0) item.mark(a, tile, ROWS, h, G, 256);
     int rpos[NQT];
     bf16x8 qf[NQT][NC];
     int last = -1;   // the last position that any row of the tile sees
-    int own0 = 0, seq = tile.item, ctx = 0;   // own0: keys that the sequence shares with its group, which are not this launch's
-    if constexpr (!GROUPS) {
-        if (seq < a.B) {
-            ctx = (int)min((int64_t)max(a.ctx_len[seq], 0), (int64_t)a.width * a.cache.page);
-            if (a.group_start) own0 = shared_of(a, seq, lane);
-        } else {
-            own0 = -1;
-        }
-        if (own0 < 0 && a.slot0 > 0 && split == 0) {   // no group: nothing was written to the first slots
-            for (int i = threadIdx.x; i < ROWS * a.slot0; i += 256) {
-                const int R = tile.at + i % ROWS;
-                if (R < tile.toks * G)
-                    a.part_ml[(int64_t)(i / ROWS) * a.T * a.hq + (int64_t)(tile.tok0 + R / G) * a.hq + h * G + R % G] = float2{-INFINITY, 0.f};
-            }
-        }
-        own0 = max(own0, 0);
-    }
 #pragma unroll
     for (int qt = 0; qt < NQT; ++qt) {
         const int R = tile.at + 16 * qt + r;
         const bool valid = R < tile.toks * G;
         const int t = tile.tok0 + (valid ? R / G : 0), hd = h * G + R % G;
-        rpos[qt] = -1;
-        if (valid) {
-            if constexpr (GROUPS) {   // the token's sequence: the last that begins at or before it
-                int s0 = first_seq(a, tile.item), s1 = first_seq(a, tile.item + 1) - 1;
-                if (a.q_start) {
-                    while (s0 < s1) {
-                        const int mid = (s0 + s1 + 1) >> 1;
-                        if (first_row(a, mid) <= t) s0 = mid;
-                        else s1 = mid - 1;
-                    }
-                } else {
-                    s0 = t;
-                }
-                rpos[qt] = min(a.ctx_len[s0], a.width * a.cache.page) - first_row(a, s0 + 1) + t;
-            } else {
-                rpos[qt] = ctx - tile.toks + (t - tile.tok0);
-            }
-        }
+        rpos[qt] = valid ? item.sees(a, tile, t) : -1;
         last = max(last, rpos[qt]);
         const uint16_t* qp = a.q + t * a.q_stride + (int64_t)hd * D;
 #pragma unroll
@@ -286,20 +344,9 @@ __global__ void __launch_bounds__(256, NQT <= 2 ? 2 : 1) quant_rows_kernel(const
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) last = max(last, __shfl_xor(last, o, 64));
     last = __builtin_amdgcn_readfirstlane(last);
-    int k0, k1;   // this tile's keys
-    if constexpr (GROUPS) {
-        k0 = 0;
-        k1 = min(shared_keys(a, tile.item), last + 1);
-        seq = min(first_seq(a, tile.item), a.B - 1);
-    } else {
-        k0 = min(own0, ctx);
-        k1 = min(ctx, last + 1);
-    }
-    const int n = max(k1 - k0, 0);
-    int chunk = (n + a.splits - 1) / a.splits;
-    chunk = max((chunk + 127) & ~127, 128);
-    const int ks = k0 + split * chunk, ke = min(k1, ks + chunk);
-    const int32_t* bt = a.bt + (int64_t)(seq < a.B ? seq : 0) * a.bt_stride;
+    int ks, ke;
+    item.piece(a, tile, last, split, 128, ks, ke);
+    const int32_t* bt = a.bt + (int64_t)item.seq * a.bt_stride;
 
     float m[NQT], l[NQT];
     f32x4 o[NQT][ND];
@@ -311,7 +358,8 @@ __global__ void __launch_bounds__(256, NQT <= 2 ? 2 : 1) quant_rows_kernel(const
         for (int dt = 0; dt < ND; ++dt) o[qt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    auto compute = [&](int t0, Step<KIND, D>& s) {
+    float unit = 0x1p-100f;   // int8: probabilities times value scales are held in float16 as 2^14 / unit of themselves; no scale so far is over it
+    auto compute = [&](int t0, const Pages& pg, Step<KIND, D>& s) {
         f32x4 sc[NQT][2];
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
@@ -324,7 +372,7 @@ __global__ void __launch_bounds__(256, NQT <= 2 ? 2 : 1) quant_rows_kernel(const
                 for (int qt = 0; qt < NQT; ++qt) sc[qt][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[qt][c], sc[qt][g], 0, 0, 0);
             }
         }
-        uint32_t nan = 0;   // keys of this lane whose values are NaN, bit 4 g + i
+        uint32_t nan = 0;   // mxfp4: keys of this lane whose values are NaN, bit 4 g + i
         if constexpr (KIND == kFp4) {
             uint32_t big = 0;   // E of 192 and more does not come from numbers: looked for in all keys at once
 #pragma unroll
@@ -340,65 +388,79 @@ __global__ void __launch_bounds__(256, NQT <= 2 ? 2 : 1) quant_rows_kernel(const
                         }
             }
         }
-        float kmul[2][4];
+        bool there[8];   // keys of this lane: there, and before the end
+        float kmul[8], vmul[8];
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+        for (int j = 0; j < 8; ++j) {
+            there[j] = pg.blk[j >> 2] >= 0 && t0 + 16 * (j >> 2) + 4 * h4 + (j & 3) < ke;
+            kmul[j] = KIND == kInt8 ? s.ks[j >> 2][j & 3] * a.scale_log2 : a.scale_log2;
+        }
+        float grown = 1.f;
+        if constexpr (KIND == kInt8) {
+            float top = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) kmul[g][i] = KIND == kInt8 ? s.ks[g][i] * a.scale_log2 : a.scale_log2;
-        bf16x8 vf[ND];
-        value_operands<KIND, D>(s, r, vf);
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, there[j] ? s.vs[j >> 2][j & 3] : 0.f);
+            if (__ballot(top > unit)) {
+                top = 2.f * rows_max(top);
+                grown = unit / top;
+                unit = top;
+            }
+            const float up = 16384.f / unit;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) vmul[j] = s.vs[j >> 2][j & 3] * up;
+        }
+        Values<KIND, D> val;
+        val.make(s, r);
 #pragma unroll
         for (int qt = 0; qt < NQT; ++qt) {
             float mx = -INFINITY;
+            bool seen[8];
 #pragma unroll
-            for (int g = 0; g < 2; ++g)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int tok = t0 + 16 * g + 4 * h4 + i;
-                    const bool seen = s.ok[g] && tok < ke && tok <= rpos[qt];
-                    const float v = seen ? sc[qt][g][i] * kmul[g][i] : -INFINITY;
-                    sc[qt][g][i] = v;
-                    mx = fmaxf(mx, v);
-                }
+            for (int j = 0; j < 8; ++j) {
+                seen[j] = there[j] && t0 + 16 * (j >> 2) + 4 * h4 + (j & 3) <= rpos[qt];
+                const float v = seen[j] ? sc[qt][j >> 2][j & 3] * kmul[j] : -INFINITY;
+                sc[qt][j >> 2][j & 3] = v;
+                mx = fmaxf(mx, v);
+            }
             mx = fmaxf(m[qt], rows_max(mx));
             const float base = mx == -INFINITY ? 0.f : mx;
             const float alpha = __builtin_amdgcn_exp2f(m[qt] - base);
             m[qt] = mx;
-            float ps = 0.f;
-            bf16x8 pf;
+            float ps = 0.f, p[8];
 #pragma unroll
-            for (int g = 0; g < 2; ++g)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float p = __builtin_amdgcn_exp2f(sc[qt][g][i] - base);
-                    const bool seen = s.ok[g] && t0 + 16 * g + 4 * h4 + i < ke && t0 + 16 * g + 4 * h4 + i <= rpos[qt];
-                    if constexpr (KIND == kFp4) {
-                        if (nan >> (4 * g + i) & 1) p = seen ? __builtin_nanf("") : 0.f;
-                    }
-                    ps += p;
-                    if constexpr (KIND == kInt8) p = seen ? p * s.vs[g][i] : 0.f;
-                    pf[4 * g + i] = (__bf16)p;
+            for (int j = 0; j < 8; ++j) {
+                p[j] = __builtin_amdgcn_exp2f(sc[qt][j >> 2][j & 3] - base);
+                if constexpr (KIND == kFp4) {
+                    if (nan >> j & 1) p[j] = seen[j] ? __builtin_nanf("") : 0.f;
                 }
-            l[qt] = l[qt] * alpha + ps;
-#pragma unroll
-            for (int dt = 0; dt < ND; ++dt) {
-                o[qt][dt] *= alpha;
-                o[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[dt], pf, o[qt][dt], 0, 0, 0);
+                ps += p[j];
+                if constexpr (KIND == kInt8) p[j] = seen[j] ? p[j] * vmul[j] : 0.f;
             }
+            l[qt] = l[qt] * alpha + ps;
+            const uint32_t pw[4] = {round2<KIND>(p[0], p[1]), round2<KIND>(p[2], p[3]), round2<KIND>(p[4], p[5]), round2<KIND>(p[6], p[7])};
+            const float old = alpha * grown;
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) o[qt][dt] = val.mul(dt, pw, o[qt][dt] * old);
         }
     };
 
-    {   // two steps of the wave under way
-        Step<KIND, D> A, B;
+    {
         int t0 = ks + w * 32;
-        if (t0 < ke) load_step<KIND, D>(a, bt, h, t0, ke, lane, A);
-        for (; t0 < ke; t0 += 256) {
-            if (t0 + 128 < ke) load_step<KIND, D>(a, bt, h, t0 + 128, ke, lane, B);
-            compute(t0, A);
-            if (t0 + 128 >= ke) break;
-            if (t0 + 256 < ke) load_step<KIND, D>(a, bt, h, t0 + 256, ke, lane, A);
-            compute(t0 + 128, B);
+        Pages pg = find_pages(a, bt, t0, ke);
+        for (; t0 < ke; t0 += 128) {
+            Step<KIND, D> s;
+            load_step<KIND, D>(a, pg, h, lane, s);
+            const Pages next = find_pages(a, bt, t0 + 128, ke);
+            compute(t0, pg, s);
+            pg = next;
         }
+    }
+    if constexpr (KIND == kInt8) {
+        const float f = unit * (1.f / (16384.f * kCodeUnit));
+#pragma unroll
+        for (int qt = 0; qt < NQT; ++qt)
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) o[qt][dt] *= f;
     }
 
     // ---- the waves' sums: those of 16 rows to the wave that has them to write ----------------------------------------------------------------------------
@@ -455,6 +517,342 @@ __global__ void __launch_bounds__(256, NQT <= 2 ? 2 : 1) quant_rows_kernel(const
                             *reinterpret_cast<f32x4*>(a.part_o + at * D + (4 * h4 + i) * ND + dt) =
                                 f32x4{o[qt][dt][i], o[qt][dt + 1][i], o[qt][dt + 2][i], o[qt][dt + 3][i]};
                 }
+            }
+        }
+    }
+}
+
+// ---- many rows: keys through LDS -------------------------------------------------------------------------------------------------------------------------
+// Tiles of 32 WAVES rows, 32 a wave, for rows that are many (prompts, the rows of a group): there the products and the probabilities bound it, and codes become operands
+// once for all waves.  A step is 16 WAVES keys: half of the waves turn its keys into bfloat16 [key][D] in LDS, the others its values into [D][key], from registers that were
+// loaded a step earlier, into the buffer that is not being read; one barrier a step.  16 bytes behind every row keep its readers, 16 bytes a lane and a row
+// each, out of each other's banks.  v_mfma_f32_32x32x16: a lane has 16 of 32 keys of one row, and the probabilities are the second product's operand as they are, its values' keys in the same order
+// (4 h + (j & 3) + 8 (j >> 2) of 16).
+// The maximum that probabilities are taken from is only moved when a score is 2^8 over it: rescaling the sums would cost as much as all else that a step does to them.
+template <int KIND, int D, int WAVES> struct TileStep {
+    static constexpr int KT = 16 * WAVES, KS = 2 * D + 16, VS = 2 * KT + 16;   // bytes from key to key, and from dimension to dimension
+    alignas(16) uint8_t k[KT * KS];
+    alignas(16) uint8_t v[D * VS];
+    alignas(16) float km[KT], vm[KT];   // int8: scales of keys, times scale_log2, and values; 0 where a key is not there
+    uint32_t there[KT / 32], nan[KT / 32];
+    float top[KT / 32];                 // int8: largest of vm
+};
+
+// 32 keys' codes on their way into LDS, by one wave: keys or values
+template <int KIND, int D> struct Fetch {
+    static constexpr int RB = row_bytes<KIND, D>(), NP = RB * 32 / 1024;   // pieces of 1 KiB
+    static constexpr int VW = Step<KIND, D>::VW;
+    uint32_t w[8 * VW > 4 * NP ? 8 * VW : 4 * NP];   // keys: 4 words of each piece; values: VW of each key
+    uint32_t e[KIND == kFp4 ? 8 : 1];                // mxfp4: E of the pieces' blocks, or the words of the eight keys' values
+    uint32_t scale;                                  // keys' waves, int8: lane i < 32: of key i, i >= 32: its value's; mxfp4: the word of key i's value
+    Pages pg;
+    int t0;
+
+    __device__ __forceinline__ int64_t row_of(const AttnArgs& a, int g, int h) const { return ((int64_t)max(pg.blk[g], 0) * a.cache.heads + h) * a.cache.page + pg.off[g]; }
+    __device__ __forceinline__ void keys(const AttnArgs& a, const int32_t* bt, int at, int end, int h, int lane) {
+        t0 = at;
+        pg = find_pages(a, bt, at, end);
+        const int64_t row0 = row_of(a, 0, h), row1 = row_of(a, 1, h);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            constexpr int KP = 1024 / RB;   // keys of a piece
+            const int key = p * KP + lane / (RB / 16);
+            const int64_t row = (NP == 1 ? key < 16 : p * KP < 16) ? row0 + key : row1 + key - 16;
+            const uint4 x = *reinterpret_cast<const uint4*>(a.cache.k + row * RB + (lane % (RB / 16)) * 16);
+            w[4 * p] = x.x, w[4 * p + 1] = x.y, w[4 * p + 2] = x.z, w[4 * p + 3] = x.w;
+            if constexpr (KIND == kFp4) e[p] = *(reinterpret_cast<const uint8_t*>(a.cache.ks) + row * (D / 32) + lane % (RB / 16));
+        }
+        const int key = lane & 31;
+        const int64_t row = key < 16 ? row0 + key : row1 + key - 16;
+        if constexpr (KIND == kInt8) scale = reinterpret_cast<const uint32_t*>(lane < 32 ? a.cache.ks : a.cache.vs)[row];
+        else if constexpr (D == 128) scale = reinterpret_cast<const uint32_t*>(a.cache.vs)[row];
+        else scale = reinterpret_cast<const uint16_t*>(a.cache.vs)[row];
+    }
+    __device__ __forceinline__ void values(const AttnArgs& a, const int32_t* bt, int at, int end, int h, int lane) {
+        t0 = at;
+        pg = find_pages(a, bt, at, end);
+        const int r = lane & 15, h2 = lane >> 4 & 1;
+        const int64_t row = (lane < 32 ? row_of(a, 0, h) : row_of(a, 1, h)) + 4 * h2;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint8_t* vp = a.cache.v + (row + (j & 3) + 8 * (j >> 2)) * RB + (RB / 16) * r;
+            if constexpr (RB == 128) {
+                const uint2 x = *reinterpret_cast<const uint2*>(vp);
+                w[VW * j] = x.x, w[VW * j + 1] = x.y;
+            } else if constexpr (RB == 64) {
+                w[VW * j] = *reinterpret_cast<const uint32_t*>(vp);
+            } else {
+                w[VW * j] = *reinterpret_cast<const uint16_t*>(vp);
+            }
+        }
+        if constexpr (KIND == kFp4) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const uint8_t* ep = reinterpret_cast<const uint8_t*>(a.cache.vs) + (row + 8 * g) * (D / 32);
+                if constexpr (D == 128) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(ep);
+                    e[4 * g] = x.x, e[4 * g + 1] = x.y, e[4 * g + 2] = x.z, e[4 * g + 3] = x.w;
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2*>(ep);
+                    e[4 * g] = x.x & 0xffff, e[4 * g + 1] = x.x >> 16, e[4 * g + 2] = x.y & 0xffff, e[4 * g + 3] = x.y >> 16;
+                }
+            }
+        }
+    }
+    // keys 32 i .. of the step
+    template <int WAVES> __device__ __forceinline__ void put_keys(TileStep<KIND, D, WAVES>& s, int i, int end, float scale_log2, int lane) const {
+        const uint32_t in = t0 >= end ? 0u : end - t0 >= 32 ? ~0u : (1u << (end - t0)) - 1u;
+        const uint32_t there = in & ((pg.blk[0] >= 0 ? 0xffffu : 0u) | (pg.blk[1] >= 0 ? 0xffff0000u : 0u));
+        const int key = lane & 31;
+        const bool here = there >> key & 1;
+        if constexpr (KIND == kInt8) {
+            const float x = here ? __uint_as_float(scale) : 0.f;
+            if (lane < 32) s.km[32 * i + key] = x * scale_log2;
+            else s.vm[32 * i + key] = x;
+            const float top = wave_max(lane < 32 ? 0.f : x);
+            if (lane == 0) s.top[i] = top, s.there[i] = there, s.nan[i] = 0;
+        } else {
+            bool bad = false;
+#pragma unroll
+            for (int b = 0; b < D / 32; ++b) bad |= (scale >> (8 * b) & 255) > 252;
+            const uint32_t nan = (uint32_t)__ballot(bad && here && lane < 32);
+            if (lane == 0) s.there[i] = there, s.nan[i] = nan;
+        }
+        constexpr int KP = 1024 / RB;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const int at = 32 * i + p * KP + lane / (RB / 16), part = lane % (RB / 16);
+            if constexpr (KIND == kInt8) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) *reinterpret_cast<bf16x8*>(s.k + at * s.KS + (2 * part + x) * 16) = eight(w[4 * p + 2 * x], w[4 * p + 2 * x + 1]);
+            } else {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    bf16x2 b[4];
+                    codes4(w[4 * p + x], __uint_as_float(e[p] << 23), b);
+                    *reinterpret_cast<bf16x8*>(s.k + at * s.KS + (4 * part + x) * 16) = bf16x8{b[0][0], b[0][1], b[1][0], b[1][1], b[2][0], b[2][1], b[3][0], b[3][1]};
+                }
+            }
+        }
+    }
+    template <int WAVES> __device__ __forceinline__ void put_values(TileStep<KIND, D, WAVES>& s, int i, int lane) const {
+        const int r = lane & 15;
+        Step<KIND, D> st;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+#pragma unroll
+            for (int x = 0; x < VW; ++x) st.v[j][x] = w[VW * j + x];
+            if constexpr (KIND == kFp4) {
+                const uint32_t one = e[j] >> (8 * (r * (D / 16) / 32)) & 255;
+                st.ve[j] = (one > 252 ? 0 : one) << (8 * (r * (D / 16) / 32));
+            }
+        }
+        Values<KIND, D> val;
+        val.make(st, r);
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt)
+            *reinterpret_cast<uint4*>(s.v + (16 * dt + r) * s.VS + (4 * i + (lane >> 4)) * 16) = uint4{val.w[dt][0], val.w[dt][1], val.w[dt][2], val.w[dt][3]};
+    }
+};
+
+template <int KIND, int D, int WAVES, bool GROUPS>
+__global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArgs a) {
+    constexpr int ROWS = 32 * WAVES, KT = 16 * WAVES, NC = D / 16, NT = D / 32;
+    typedef TileStep<KIND, D, WAVES> TS;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    TS* steps = reinterpret_cast<TS*>(lds);
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 31, h2 = lane >> 5;
+    const int heads = a.cache.heads, G = a.hq / heads;
+    const int h = blockIdx.x % heads, split = blockIdx.y;
+    Tile tile;
+    if (!find_tile<GROUPS>(a, blockIdx.x / heads, G, ROWS, lane, tile)) return;
+    const Item<GROUPS> item(a, tile, lane);
+    if (split == 0) item.mark(a, tile, ROWS, h, G, 64 * WAVES);
+
+    const int R = tile.at + 32 * w + r, live_rows = tile.toks * G;
+    const bool valid = R < live_rows;
+    const int t = tile.tok0 + (valid ? R / G : 0);
+    const int rpos = valid ? item.sees(a, tile, t) : -1;
+    bf16x8 qf[NC];
+    {
+        const uint16_t* qp = a.q + t * a.q_stride + (int64_t)(h * G + R % G) * D + 8 * h2;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            qf[c] = *reinterpret_cast<const bf16x8*>(qp + 16 * c);
+            if (!valid) qf[c] = bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
+        }
+    }
+    int first = valid ? rpos : INT_MAX, last = rpos;   // of the wave's rows
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        first = min(first, __shfl_xor(first, o, 64));
+        last = max(last, __shfl_xor(last, o, 64));
+    }
+    first = __builtin_amdgcn_readfirstlane(first);
+    last = __builtin_amdgcn_readfirstlane(last);
+    int all;   // the last that any row of the tile sees
+    {
+        int* seen = reinterpret_cast<int*>(lds);
+        if (lane == 0) seen[w] = last;
+        __syncthreads();
+        all = seen[0];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) all = max(all, seen[i]);
+        all = __builtin_amdgcn_readfirstlane(all);
+        __syncthreads();
+    }
+    int ks, ke;
+    item.piece(a, tile, all, split, KT, ks, ke);
+    const int32_t* bt = a.bt + (int64_t)item.seq * a.bt_stride;
+
+    // int8: value scales so far are up to `unit`, and sums are held 2^lift = 64 / unit times as large: probabilities, up to 2^8, times scales fit float16
+    float m = -INFINITY, l = 0.f, unit = 0x1p-100f, lift = 0.f;
+    f32x16 o[NT];
+#pragma unroll
+    for (int T = 0; T < NT; ++T)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[T][i] = 0.f;
+
+    const bool of_keys = w < WAVES / 2;
+    const int part = of_keys ? w : w - WAVES / 2;   // of the step's keys
+    Fetch<KIND, D> f;
+    auto fetch = [&](int at) {
+        if (of_keys) f.keys(a, bt, at + 32 * part, ke, h, lane);
+        else f.values(a, bt, at + 32 * part, ke, h, lane);
+    };
+    auto store = [&](TS& s) {
+        if (of_keys) f.template put_keys<WAVES>(s, part, ke, a.scale_log2, lane);
+        else f.template put_values<WAVES>(s, part, lane);
+    };
+
+    // 32 keys from t0 on, the step's sub-th
+    auto compute = [&](const TS& s, int sub, int t0, auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;   // every row sees every key, and none has values that are NaN
+        f32x16 sc;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(s.k + (32 * sub + r) * TS::KS + (2 * c + h2) * 16), qf[c], sc, 0, 0, 0);
+        float km[16];
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const f32x4 x = KIND == kInt8 ? *reinterpret_cast<const f32x4*>(s.km + 32 * sub + 4 * h2 + 2 * i) : f32x4{a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2};
+            km[i] = x[0], km[i + 1] = x[1], km[i + 2] = x[2], km[i + 3] = x[3];
+        }
+        uint32_t seen = 0xffff;   // of this lane's keys: bit i is key 4 h2 + (i & 3) + 8 (i >> 2)
+        uint32_t nan = 0;
+        if constexpr (!WHOLE) {
+            const uint32_t row = rpos < t0 ? 0u : rpos - t0 >= 31 ? ~0u : (2u << (rpos - t0)) - 1u;
+            const uint32_t k = (s.there[sub] & row) >> (4 * h2);
+            seen = (k & 15) | (k >> 4 & 0xf0) | (k >> 8 & 0xf00) | (k >> 12 & 0xf000);
+            const uint32_t n = s.nan[sub] >> (4 * h2);
+            nan = (n & 15) | (n >> 4 & 0xf0) | (n >> 8 & 0xf00) | (n >> 12 & 0xf000);
+        }
+        float base = m == -INFINITY ? -lift : m - lift, x[16], mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            x[i] = __builtin_fmaf(sc[i], km[i], -base);
+            if constexpr (!WHOLE) x[i] = seen >> i & 1 ? x[i] : -INFINITY;
+            mx = fmaxf(mx, x[i]);
+        }
+        mx = lanes_xor32(mx, LaneMax{});
+        float top = 0.f;
+        if constexpr (KIND == kInt8) top = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(s.top[sub])));
+        if (__ballot(mx > (m == -INFINITY ? -INFINITY : lift + 8.f)) || top > unit) {
+            const float to = mx > -INFINITY ? fmaxf(mx + base, m) : m, from = m - lift;
+            if (top > unit) {
+                unit = 2.f * top;
+                lift = __log2f(64.f / unit);
+            }
+            const float now = to == -INFINITY ? -lift : to - lift, old = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(from - now), d = base - now;
+            m = to;
+            l *= old;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] += d;
+#pragma unroll
+            for (int T = 0; T < NT; ++T) o[T] *= old;
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {   // 16 keys: probabilities, and their part of the sums
+            uint32_t pw[4];
+            f32x4 vm[2];
+            if constexpr (KIND == kInt8) {
+                vm[0] = *reinterpret_cast<const f32x4*>(s.vm + 32 * sub + 16 * kk + 4 * h2);
+                vm[1] = *reinterpret_cast<const f32x4*>(s.vm + 32 * sub + 16 * kk + 4 * h2 + 8);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                float p[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int i = 8 * kk + j + e;
+                    p[e] = __builtin_amdgcn_exp2f(x[i]);
+                    if constexpr (!WHOLE && KIND == kFp4) {
+                        if (nan >> i & 1) p[e] = seen >> i & 1 ? __builtin_nanf("") : 0.f;
+                    }
+                    l += p[e];
+                    if constexpr (KIND == kInt8) p[e] = WHOLE || (seen >> i & 1) ? p[e] * vm[j >> 2][(j & 3) + e] : 0.f;
+                }
+                pw[j >> 1] = round2<KIND>(p[0], p[1]);
+            }
+            const uint4 p{pw[0], pw[1], pw[2], pw[3]};
+#pragma unroll
+            for (int T = 0; T < NT; ++T) {
+                const uint4 v = *reinterpret_cast<const uint4*>(s.v + (32 * T + r) * TS::VS + (4 * sub + 2 * kk + h2) * 16);
+                if constexpr (KIND == kInt8) o[T] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v), __builtin_bit_cast(f16x8, p), o[T], 0, 0, 0);
+                else o[T] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, p), o[T], 0, 0, 0);
+            }
+        }
+    };
+
+    if (ks < ke) {
+        fetch(ks);
+        store(steps[0]);
+        __syncthreads();
+        int b = 0;
+        for (int t0 = ks; t0 < ke; t0 += KT, b ^= 1) {
+            const bool more = t0 + KT < ke;
+            if (more) fetch(t0 + KT);
+            const TS& s = steps[b];
+#pragma unroll 1
+            for (int sub = 0; sub < KT / 32; ++sub) {
+                const int at = t0 + 32 * sub;
+                if (at > last || at >= ke) break;   // no row of the wave sees these
+                const bool whole = __builtin_amdgcn_readfirstlane(~s.there[sub] | s.nan[sub]) == 0 && at + 31 <= first;
+                if (whole) compute(s, sub, at, std::true_type{});
+                else compute(s, sub, at, std::false_type{});
+            }
+            if (more) store(steps[b ^ 1]);
+            __syncthreads();
+        }
+    }
+
+    l = lanes_xor32(l, LaneSum{});
+    if (!valid) return;
+    const float mul = KIND == kInt8 ? 1.f / kCodeUnit : 1.f;
+    const int64_t row = (int64_t)t * a.hq + h * G + R % G;
+    if (a.slots == 1) {
+        const float inv = l == 0.f ? 0.f : mul / l;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {   // row 32 T + (i & 3) + 8 (i >> 2) + 4 h2 of V is dimension D / 16 (row % 16) + row / 16
+            uint16_t* dst = a.out + row * D + ((i & 3) + 8 * (i >> 2) + 4 * h2) * (D / 16);
+            uint16_t v[2 * NT];
+#pragma unroll
+            for (int T = 0; T < NT; ++T) v[2 * T] = f2bf(o[T][i] * inv), v[2 * T + 1] = f2bf(o[T][i + 8] * inv);
+            if constexpr (NT == 4) *reinterpret_cast<u16x8*>(dst) = u16x8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+            else *reinterpret_cast<u16x4*>(dst) = u16x4{v[0], v[1], v[2], v[3]};
+        }
+    } else {
+        const int64_t at = (int64_t)(a.slot0 + split) * a.T * a.hq + row;
+        if (h2 == 0) a.part_ml[at] = float2{m - lift, l};
+        if (l != 0.f) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float* dst = a.part_o + at * D + ((i & 3) + 8 * (i >> 2) + 4 * h2) * (D / 16);
+#pragma unroll
+                for (int T = 0; T < NT; T += 2) *reinterpret_cast<f32x4*>(dst + 2 * T) = f32x4{o[T][i], o[T][i + 8], o[T + 1][i], o[T + 1][i + 8]} * mul;
             }
         }
     }
@@ -519,23 +917,35 @@ __global__ void __launch_bounds__(256) quant_join_kernel(const float* __restrict
     *reinterpret_cast<u16x4*>(out + row * D + 4 * c) = u16x4{f2bf(o[0] * inv), f2bf(o[1] * inv), f2bf(o[2] * inv), f2bf(o[3] * inv)};
 }
 
-template <int KIND, int D, bool GROUPS> void launch_rows(int nqt, const AttnArgs& a, int64_t tiles, hipStream_t st) {
+template <int KIND, int D, bool GROUPS> void launch_rows(int rows, const AttnArgs& a, int64_t tiles, hipStream_t st) {
     const dim3 g((unsigned)(tiles * a.cache.heads), a.splits), b(256);
-    if (nqt == 1) hipLaunchKernelGGL((quant_rows_kernel<KIND, D, 1, GROUPS>), g, b, 0, st, a);
-    else if (nqt == 2) hipLaunchKernelGGL((quant_rows_kernel<KIND, D, 2, GROUPS>), g, b, 0, st, a);
-    else hipLaunchKernelGGL((quant_rows_kernel<KIND, D, 4, GROUPS>), g, b, 0, st, a);
+    if (rows == 16) {
+        hipLaunchKernelGGL((quant_rows_kernel<KIND, D, 1, GROUPS>), g, b, 0, st, a);
+    } else if (rows == 32) {
+        hipLaunchKernelGGL((quant_rows_kernel<KIND, D, 2, GROUPS>), g, b, 0, st, a);
+    } else if (rows == 128) {
+        constexpr int lds = 2 * sizeof(TileStep<KIND, D, 4>);
+        lds_limit<quant_tile_kernel<KIND, D, 4, GROUPS>>(lds);
+        hipLaunchKernelGGL((quant_tile_kernel<KIND, D, 4, GROUPS>), g, b, lds, st, a);
+    } else {
+        constexpr int lds = 2 * sizeof(TileStep<KIND, D, 8>);
+        lds_limit<quant_tile_kernel<KIND, D, 8, GROUPS>>(lds);
+        hipLaunchKernelGGL((quant_tile_kernel<KIND, D, 8, GROUPS>), g, dim3(512), lds, st, a);
+    }
 }
-template <bool GROUPS> void launch_rows_of(int kind, int D, int nqt, const AttnArgs& a, int64_t tiles, hipStream_t st) {
-    if (kind == kInt8 && D == 64) launch_rows<kInt8, 64, GROUPS>(nqt, a, tiles, st);
-    else if (kind == kInt8) launch_rows<kInt8, 128, GROUPS>(nqt, a, tiles, st);
-    else if (D == 64) launch_rows<kFp4, 64, GROUPS>(nqt, a, tiles, st);
-    else launch_rows<kFp4, 128, GROUPS>(nqt, a, tiles, st);
+template <bool GROUPS> void launch_rows_of(int kind, int D, int rows, const AttnArgs& a, int64_t tiles, hipStream_t st) {
+    if (kind == kInt8 && D == 64) launch_rows<kInt8, 64, GROUPS>(rows, a, tiles, st);
+    else if (kind == kInt8) launch_rows<kInt8, 128, GROUPS>(rows, a, tiles, st);
+    else if (D == 64) launch_rows<kFp4, 64, GROUPS>(rows, a, tiles, st);
+    else launch_rows<kFp4, 128, GROUPS>(rows, a, tiles, st);
 }
 
 // Rows of a tile, by the rows that an item has on average
-int tiles_of(int64_t rows, int64_t items) {
+int tile_of(int64_t rows, int64_t items) {
     const int64_t per = items > 0 ? rows / items : rows;
-    return per <= 16 ? 1 : per <= 32 ? 2 : 4;
+    const int k = knob("qrows", 0);
+    if (k && per > 32) return k;
+    return per <= 16 ? 16 : per <= 32 ? 32 : per <= 128 ? 128 : 256;
 }
 
 }  // namespace
@@ -544,16 +954,17 @@ int tiles_of(int64_t rows, int64_t items) {
 AttnPlan quant_attention_plan(int T, int B, int groups, int hq, int heads, int64_t keys) {
     AttnPlan p{};
     const int64_t rows = (int64_t)T * (hq / heads);
-    auto side = [&](int64_t items, int& nqt, int64_t& tiles, int& splits) {
-        nqt = tiles_of(rows, items);
-        tiles = rows / (16 * nqt) + items + 1;
-        const int64_t wgs = ((rows + 16 * nqt - 1) / (16 * nqt) > items ? (rows + 16 * nqt - 1) / (16 * nqt) : items) * heads;
-        int64_t s = (1024 + wgs - 1) / wgs;
-        s = s < (keys + 255) / 256 ? s : (keys + 255) / 256;
+    auto side = [&](int64_t items, int& tile, int64_t& tiles, int& splits) {
+        tile = tile_of(rows, items);
+        tiles = rows / tile + items + 1;
+        const int64_t wgs = ((rows + tile - 1) / tile > items ? (rows + tile - 1) / tile : items) * heads;
+        const int64_t target = tile <= 32 ? knob("qat", 1024) : tile == 128 ? knob("qtt", 512) : knob("qtt", 512) / 2, least = tile <= 32 ? 256 : tile;
+        int64_t s = tile <= 32 ? (target + wgs - 1) / wgs : (target + wgs / 2) / wgs;
+        s = s < (keys + least - 1) / least ? s : (keys + least - 1) / least;
         splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
     };
-    side(B, p.own_nqt, p.own_tiles, p.own_splits);
-    if (groups > 0) side(groups, p.group_nqt, p.group_tiles, p.group_splits);
+    side(B, p.own_rows, p.own_tiles, p.own_splits);
+    if (groups > 0) side(groups, p.group_rows, p.group_tiles, p.group_splits);
     p.slots = p.own_splits + p.group_splits;
     return p;
 }
@@ -563,17 +974,18 @@ void launch_quant_attention(int kind, int D, const AttnPlan& p, const uint16_t* 
                             float scale, uint16_t* out, float* part_o, float* part_ml, hipStream_t st) {
     if (T == 0) return;
     AttnArgs a{q, q_stride, cache, bt, bt_stride, width, q_start, ctx_len, groups ? group_start : nullptr, prefix_len, B, T, groups, hq, scale * 1.4426950408889634f,
-               out, part_o, reinterpret_cast<float2*>(part_ml), p.slots, 0, 0};
+               out, part_o, reinterpret_cast<float2*>(part_ml), p.slots, 0, 0,
+               (cache.page & (cache.page - 1)) ? -1 : __builtin_ctz(cache.page)};
     if (groups) {
         a.splits = p.group_splits;
         a.slot0 = 0;
-        launch_rows_of<true>(kind, D, p.group_nqt, a, p.group_tiles, st);
+        launch_rows_of<true>(kind, D, p.group_rows, a, p.group_tiles, st);
     }
     a.splits = p.own_splits;
     a.slot0 = p.group_splits;
     // one token of each sequence: tiles are counted without a look at where sequences begin
-    const int64_t tiles = q_start ? p.own_tiles : (int64_t)T * ((hq / cache.heads + 16 * p.own_nqt - 1) / (16 * p.own_nqt));
-    launch_rows_of<false>(kind, D, p.own_nqt, a, tiles, st);
+    const int64_t tiles = q_start ? p.own_tiles : (int64_t)T * ((hq / cache.heads + p.own_rows - 1) / p.own_rows);
+    launch_rows_of<false>(kind, D, p.own_rows, a, tiles, st);
     if (p.slots > 1) {
         const int64_t rows = (int64_t)T * hq;
         const int gr = 256 / (D / 4);
