@@ -606,11 +606,14 @@ template <int KIND, int D> struct Fetch {
         const int key = lane & 31;
         const bool here = there >> key & 1;
         if constexpr (KIND == kInt8) {
-            const float x = here ? __uint_as_float(scale) : 0.f;
+            float x = here ? __uint_as_float(scale) : 0.f;
+            const bool bad = lane >= 32 && !(x < INFINITY);
+            if (bad) x = 0.f;
             if (lane < 32) s.km[32 * i + key] = x * scale_log2;
             else s.vm[32 * i + key] = x;
             const float top = wave_max(lane < 32 ? 0.f : x);
-            if (lane == 0) s.top[i] = top, s.there[i] = there, s.nan[i] = 0;
+            const uint32_t nan = (uint32_t)(__ballot(bad) >> 32);
+            if (lane == 0) s.top[i] = top, s.there[i] = there, s.nan[i] = nan;
         } else {
             bool bad = false;
 #pragma unroll
@@ -707,7 +710,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
     const int32_t* bt = a.bt + (int64_t)item.seq * a.bt_stride;
 
     // int8: value scales so far are up to `unit`, and sums are held 2^lift = 64 / unit times as large: probabilities, up to 2^8, times scales fit float16
-    float m = -INFINITY, l = 0.f, unit = 0x1p-100f, lift = 0.f;
+    float m = -INFINITY, l = 0.f, unit = KIND == kInt8 ? 0x1p-100f : 0.f, lift = 0.f;
     f32x16 o[NT];
 #pragma unroll
     for (int T = 0; T < NT; ++T)
@@ -727,40 +730,37 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
     };
 
     // 32 keys from t0 on, the step's sub-th
-    auto compute = [&](const TS& s, int sub, int t0, auto whole) {
-        constexpr bool WHOLE = decltype(whole)::value;   // every row sees every key, and none has values that are NaN
+    auto compute = [&](const TS& s, int sub, int t0) {
         f32x16 sc;
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
             sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(s.k + (32 * sub + r) * TS::KS + (2 * c + h2) * 16), qf[c], sc, 0, 0, 0);
-        float km[16];
+        const float base = m == -INFINITY ? -lift : m - lift;
+        float x[16], mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
-            const f32x4 x = KIND == kInt8 ? *reinterpret_cast<const f32x4*>(s.km + 32 * sub + 4 * h2 + 2 * i) : f32x4{a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2};
-            km[i] = x[0], km[i + 1] = x[1], km[i + 2] = x[2], km[i + 3] = x[3];
-        }
-        uint32_t seen = 0xffff;   // of this lane's keys: bit i is key 4 h2 + (i & 3) + 8 (i >> 2)
-        uint32_t nan = 0;
-        if constexpr (!WHOLE) {
-            const uint32_t row = rpos < t0 ? 0u : rpos - t0 >= 31 ? ~0u : (2u << (rpos - t0)) - 1u;
-            const uint32_t k = (s.there[sub] & row) >> (4 * h2);
-            seen = (k & 15) | (k >> 4 & 0xf0) | (k >> 8 & 0xf00) | (k >> 12 & 0xf000);
-            const uint32_t n = s.nan[sub] >> (4 * h2);
-            nan = (n & 15) | (n >> 4 & 0xf0) | (n >> 8 & 0xf00) | (n >> 12 & 0xf000);
-        }
-        float base = m == -INFINITY ? -lift : m - lift, x[16], mx = -INFINITY;
+            const f32x4 km = KIND == kInt8 ? *reinterpret_cast<const f32x4*>(s.km + 32 * sub + 4 * h2 + 2 * i) : f32x4{a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            x[i] = __builtin_fmaf(sc[i], km[i], -base);
-            if constexpr (!WHOLE) x[i] = seen >> i & 1 ? x[i] : -INFINITY;
-            mx = fmaxf(mx, x[i]);
+            for (int e = 0; e < 4; ++e) x[i + e] = __builtin_fmaf(sc[i + e], km[e], -base);
         }
+        const uint32_t there = __builtin_amdgcn_readfirstlane(s.there[sub]), nans = __builtin_amdgcn_readfirstlane(s.nan[sub]);
+        if (t0 + 31 > first || (~there | nans)) {   // some row does not see some key, or a key's value is NaN
+            const uint32_t row = rpos < t0 ? 0u : rpos - t0 >= 31 ? ~0u : (2u << (rpos - t0)) - 1u;
+            const uint32_t seen = (there & row) >> (4 * h2), nan = nans >> (4 * h2);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {   // key 4 h2 + (i & 3) + 8 (i >> 2)
+                const uint32_t bit = 1u << ((i & 3) + 8 * (i >> 2));
+                x[i] = !(seen & bit) ? -INFINITY : nan & bit ? __builtin_nanf("") : x[i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[i]);
         mx = lanes_xor32(mx, LaneMax{});
         float top = 0.f;
         if constexpr (KIND == kInt8) top = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(s.top[sub])));
-        if (__ballot(mx > (m == -INFINITY ? -INFINITY : lift + 8.f)) || top > unit) {
+        if (__builtin_expect(__ballot(mx > (m == -INFINITY ? -INFINITY : lift + 8.f)) != 0 || top > unit, false)) {
             const float to = mx > -INFINITY ? fmaxf(mx + base, m) : m, from = m - lift;
             if (top > unit) {
                 unit = 2.f * top;
@@ -777,25 +777,21 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {   // 16 keys: probabilities, and their part of the sums
             uint32_t pw[4];
-            f32x4 vm[2];
-            if constexpr (KIND == kInt8) {
-                vm[0] = *reinterpret_cast<const f32x4*>(s.vm + 32 * sub + 16 * kk + 4 * h2);
-                vm[1] = *reinterpret_cast<const f32x4*>(s.vm + 32 * sub + 16 * kk + 4 * h2 + 8);
-            }
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                float p[2];
+            for (int j = 0; j < 8; j += 4) {
+                float p[4];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int i = 8 * kk + j + e;
-                    p[e] = __builtin_amdgcn_exp2f(x[i]);
-                    if constexpr (!WHOLE && KIND == kFp4) {
-                        if (nan >> i & 1) p[e] = seen >> i & 1 ? __builtin_nanf("") : 0.f;
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    p[e] = __builtin_amdgcn_exp2f(x[8 * kk + j + e]);
                     l += p[e];
-                    if constexpr (KIND == kInt8) p[e] = WHOLE || (seen >> i & 1) ? p[e] * vm[j >> 2][(j & 3) + e] : 0.f;
+                }
+                if constexpr (KIND == kInt8) {
+                    const f32x4 vm = *reinterpret_cast<const f32x4*>(s.vm + 32 * sub + 16 * kk + 4 * h2 + 2 * j);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[e] *= vm[e];
                 }
                 pw[j >> 1] = round2<KIND>(p[0], p[1]);
+                pw[(j >> 1) + 1] = round2<KIND>(p[2], p[3]);
             }
             const uint4 p{pw[0], pw[1], pw[2], pw[3]};
 #pragma unroll
@@ -815,46 +811,52 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
         for (int t0 = ks; t0 < ke; t0 += KT, b ^= 1) {
             const bool more = t0 + KT < ke;
             if (more) fetch(t0 + KT);
-            const TS& s = steps[b];
 #pragma unroll 1
             for (int sub = 0; sub < KT / 32; ++sub) {
                 const int at = t0 + 32 * sub;
                 if (at > last || at >= ke) break;   // no row of the wave sees these
-                const bool whole = __builtin_amdgcn_readfirstlane(~s.there[sub] | s.nan[sub]) == 0 && at + 31 <= first;
-                if (whole) compute(s, sub, at, std::true_type{});
-                else compute(s, sub, at, std::false_type{});
+                compute(steps[b], sub, at);
             }
             if (more) store(steps[b ^ 1]);
             __syncthreads();
         }
     }
 
+    // Sums to memory, by way of LDS (the wave's rows in its own part): 16 bytes a lane, a row's in neighbouring lanes.  Row 32 T + (i & 3) + 8 (i >> 2) + 4 h2 of V is
+    // dimension D / 16 (row % 16) + row / 16: a lane has D / 16 neighbouring dimensions at a time.
     l = lanes_xor32(l, LaneSum{});
-    if (!valid) return;
-    const float mul = KIND == kInt8 ? 1.f / kCodeUnit : 1.f;
-    const int64_t row = (int64_t)t * a.hq + h * G + R % G;
-    if (a.slots == 1) {
-        const float inv = l == 0.f ? 0.f : mul / l;
+    const bool direct = a.slots == 1;
+    const float mul = (KIND == kInt8 ? 1.f / kCodeUnit : 1.f) * (direct ? (l == 0.f ? 0.f : 1.f / l) : 1.f);
+    if (!direct && h2 == 0 && valid) a.part_ml[(int64_t)(a.slot0 + split) * a.T * a.hq + (int64_t)t * a.hq + h * G + R % G] = float2{m - lift, l};
+    constexpr int OS = D + 4;   // floats from row to row
+    float* mine = reinterpret_cast<float*>(lds) + w * 16 * OS;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {   // row 32 T + (i & 3) + 8 (i >> 2) + 4 h2 of V is dimension D / 16 (row % 16) + row / 16
-            uint16_t* dst = a.out + row * D + ((i & 3) + 8 * (i >> 2) + 4 * h2) * (D / 16);
-            uint16_t v[2 * NT];
-#pragma unroll
-            for (int T = 0; T < NT; ++T) v[2 * T] = f2bf(o[T][i] * inv), v[2 * T + 1] = f2bf(o[T][i + 8] * inv);
-            if constexpr (NT == 4) *reinterpret_cast<u16x8*>(dst) = u16x8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
-            else *reinterpret_cast<u16x4*>(dst) = u16x4{v[0], v[1], v[2], v[3]};
-        }
-    } else {
-        const int64_t at = (int64_t)(a.slot0 + split) * a.T * a.hq + row;
-        if (h2 == 0) a.part_ml[at] = float2{m - lift, l};
-        if (l != 0.f) {
+    for (int half = 0; half < 2; ++half) {   // 16 rows at a time
+        if ((r >> 4) == half) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                float* dst = a.part_o + at * D + ((i & 3) + 8 * (i >> 2) + 4 * h2) * (D / 16);
+                float* dst = mine + (r & 15) * OS + ((i & 3) + 8 * (i >> 2) + 4 * h2) * (D / 16);
 #pragma unroll
                 for (int T = 0; T < NT; T += 2) *reinterpret_cast<f32x4*>(dst + 2 * T) = f32x4{o[T][i], o[T][i + 8], o[T + 1][i], o[T + 1][i + 8]} * mul;
             }
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // of this wave alone
+        constexpr int PER = D / 8;   // lanes of a row, eight dimensions each
+#pragma unroll
+        for (int i = 0; i < 16 * PER / 64; ++i) {
+            const int at = (i * 64 + lane) / PER, c = lane % PER, Rr = tile.at + 32 * w + 16 * half + at;
+            if (Rr >= live_rows) continue;
+            const int64_t row = (int64_t)(tile.tok0 + Rr / G) * a.hq + h * G + Rr % G;
+            const f32x4 x = *reinterpret_cast<const f32x4*>(mine + at * OS + 8 * c), y = *reinterpret_cast<const f32x4*>(mine + at * OS + 8 * c + 4);
+            if (direct) {
+                *reinterpret_cast<u16x8*>(a.out + row * D + 8 * c) = u16x8{f2bf(x[0]), f2bf(x[1]), f2bf(x[2]), f2bf(x[3]), f2bf(y[0]), f2bf(y[1]), f2bf(y[2]), f2bf(y[3])};
+            } else {
+                float* dst = a.part_o + ((int64_t)(a.slot0 + split) * a.T * a.hq + row) * D + 8 * c;
+                *reinterpret_cast<f32x4*>(dst) = x;
+                *reinterpret_cast<f32x4*>(dst + 4) = y;
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 }
 
