@@ -729,14 +729,18 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
         else f.template put_values<WAVES>(s, part, lane);
     };
 
-    // 32 keys from t0 on, the step's sub-th
-    auto compute = [&](const TS& s, int sub, int t0) {
+    auto scores = [&](const TS& s, int sub) {
         f32x16 sc;
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
             sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(s.k + (32 * sub + r) * TS::KS + (2 * c + h2) * 16), qf[c], sc, 0, 0, 0);
+        return sc;
+    };
+    // 32 keys from t0 on, the step's sub-th, whose scores are made; makes the next ones' beside the probabilities
+    f32x16 sc;
+    auto compute = [&](const TS& s, int sub, int t0) {
         const float base = m == -INFINITY ? -lift : m - lift;
         float x[16], mx = -INFINITY;
 #pragma unroll
@@ -774,6 +778,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
 #pragma unroll
             for (int T = 0; T < NT; ++T) o[T] *= old;
         }
+        if (sub + 1 < KT / 32) sc = scores(s, sub + 1);
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {   // 16 keys: probabilities, and their part of the sums
             uint32_t pw[4];
@@ -811,11 +816,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
         for (int t0 = ks; t0 < ke; t0 += KT, b ^= 1) {
             const bool more = t0 + KT < ke;
             if (more) fetch(t0 + KT);
-#pragma unroll 1
-            for (int sub = 0; sub < KT / 32; ++sub) {
-                const int at = t0 + 32 * sub;
-                if (at > last || at >= ke) break;   // no row of the wave sees these
-                compute(steps[b], sub, at);
+            if (t0 <= last) {
+                sc = scores(steps[b], 0);
+#pragma unroll
+                for (int sub = 0; sub < KT / 32; ++sub) {
+                    const int at = t0 + 32 * sub;
+                    if (at > last || at >= ke) break;   // no row of the wave sees these
+                    compute(steps[b], sub, at);
+                }
             }
             if (more) store(steps[b ^ 1]);
             __syncthreads();
