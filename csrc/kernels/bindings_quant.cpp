@@ -15,7 +15,7 @@ namespace qkv {
 void launch_norm_rope_kv_quant(int, int, const uint16_t*, int64_t, const int32_t*, const int32_t*, const int32_t*, int64_t, int, int, const float*, int, int,
                                const uint16_t*, const uint16_t*, double, uint16_t*, const Cache&, int64_t, int, hipStream_t);
 void launch_quant_kv_read(int, int, const int32_t*, const int32_t*, const int32_t*, int64_t, int, int, const Cache&, uint16_t*, uint16_t*, int64_t, hipStream_t);
-AttnPlan quant_attention_plan(int, int, int, int, int, int64_t);
+AttnPlan quant_attention_plan(int, int, bool, int, int, int, int64_t);
 void launch_quant_attention(int, int, const AttnPlan&, const uint16_t*, int64_t, const Cache&, const int32_t*, int64_t, int, const int32_t*, const int32_t*,
                             const int32_t*, const int32_t*, int, int, int, int, float, uint16_t*, float*, float*, hipStream_t);
 }  // namespace qkv
@@ -156,7 +156,7 @@ Tensor quant_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
     if (B == 0 || keys == 0) return out.zero_();
     const bool rows = q.stride(2) == 1 && q.stride(1) == D && q.stride(0) % 8 == 0 && q.stride(0) >= 0 && (uintptr_t)q.data_ptr() % 16 == 0;
     const Tensor x = rows ? q : q.clone(at::MemoryFormat::Contiguous);
-    const auto p = chronos::qkv::quant_attention_plan((int)T, (int)B, (int)groups, (int)hq, (int)heads, max_ctx > 0 && max_ctx < keys ? max_ctx : keys);
+    const auto p = chronos::qkv::quant_attention_plan((int)T, (int)B, qs == nullptr, (int)groups, (int)hq, (int)heads, max_ctx > 0 && max_ctx < keys ? max_ctx : keys);
     Tensor po, pm;
     if (p.slots > 1) {
         po = at::empty({p.slots, T * hq, D}, q.options().dtype(at::kFloat));

@@ -43,6 +43,7 @@ struct AttnArgs {
     float2* part_ml;          // [slots, T * hq]: maximum (base 2) and sum
     int slots, splits, slot0;
     int page_shift;           // pages of a power of two tokens; -1: others
+    int share;                // 0: every sequence's keys in `splits` pieces; else pieces of one size, about so many a key head (find_piece)
 };
 
 namespace {
@@ -60,6 +61,12 @@ struct Tile {
     int item;       // sequence or group; a.B: the tokens behind the last sequence
     int tok0, toks;   // the item's tokens
     int at;         // the tile's first row among the item's toks * G
+    __device__ __forceinline__ void same() {   // they are the same in all lanes, and the compiler may know
+        item = __builtin_amdgcn_readfirstlane(item);
+        tok0 = __builtin_amdgcn_readfirstlane(tok0);
+        toks = __builtin_amdgcn_readfirstlane(toks);
+        at = __builtin_amdgcn_readfirstlane(at);
+    }
 };
 // Tile `index` of the items' tiles of `rows` rows, in order.  Every wave finds it by itself: 64 items at a time, their tiles counted up across the lanes.
 template <bool GROUPS> __device__ __forceinline__ bool find_tile(const AttnArgs& a, int index, int G, int rows, int lane, Tile& out) {
@@ -120,8 +127,8 @@ template <bool GROUPS> struct Item {
             seq = min(first_seq(a, t.item), a.B - 1);
         } else {
             if (seq < a.B) {
-                ctx = (int)min((int64_t)max(a.ctx_len[seq], 0), (int64_t)a.width * a.cache.page);
-                if (a.group_start) k0 = shared_of(a, seq, lane);
+                ctx = __builtin_amdgcn_readfirstlane((int)min((int64_t)max(a.ctx_len[seq], 0), (int64_t)a.width * a.cache.page));
+                if (a.group_start) k0 = __builtin_amdgcn_readfirstlane(shared_of(a, seq, lane));
             } else {
                 k0 = -1;
                 seq = 0;
@@ -165,6 +172,70 @@ template <bool GROUPS> struct Item {
     }
 };
 
+// One token of each of up to 256 sequences, of lengths that may be far apart: their keys in pieces of one size, a multiple of 128 keys, for about a.share workgroups a
+// key head, at most `slots` a sequence.  Piece `index` of the sequences' pieces in order; behind them the tokens of no sequence.  Every wave counts by itself.
+struct Piece {
+    int seq, split, splits, keys;   // seq: or the token, from B on; keys: of a piece
+};
+__device__ __forceinline__ int lanes_scan(int v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(v, o, 64);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+__device__ __forceinline__ bool find_piece(const AttnArgs& a, int index, int lane, Piece& out) {
+    constexpr int CH = 4;
+    int units[CH], sum = 0, most = 0;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int seq = i * 64 + lane;
+        units[i] = seq < a.B ? (int)((min((int64_t)max(a.ctx_len[seq], 0), (int64_t)a.width * a.cache.page) + 127) >> 7) : 0;
+        sum += units[i];
+        most = max(most, units[i]);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        sum += __shfl_xor(sum, o, 64);
+        most = max(most, __shfl_xor(most, o, 64));
+    }
+    sum = __builtin_amdgcn_readfirstlane(sum);
+    most = __builtin_amdgcn_readfirstlane(most);
+    const int size = max(max((sum + a.share - 1) / a.share, (most + a.slots - 1) / a.slots), 1);
+    const float inv = 1.f / (float)size;
+    int full[CH], all = 0;   // whole pieces; they come first, the sequences' rests (also of none) when places become free
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        int n = (int)((float)units[i] * inv);   // units up to 2^23: a quotient that is off by one is put right
+        n += (n + 1) * size <= units[i];
+        full[i] = n - (n * size > units[i]);
+        all += full[i];
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) all += __shfl_xor(all, o, 64);
+    all = __builtin_amdgcn_readfirstlane(all);
+    const bool rests = index >= all;
+    int before = rests ? all : 0;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        if (i * 64 >= a.B) break;
+        const int rest = i * 64 + lane < a.B && (full[i] * size < units[i] || units[i] == 0), n = rests ? rest : full[i];
+        const int upto = lanes_scan(n, lane), total = __builtin_amdgcn_readlane(upto, 63);
+        if (index < before + total) {
+            const int l = __builtin_ctzll(__ballot(before + upto > index)), f = __builtin_amdgcn_readlane(full[i], l);
+            out.seq = i * 64 + l;
+            out.splits = f + __builtin_amdgcn_readlane(rest, l);
+            out.split = rests ? f : index - before - (__builtin_amdgcn_readlane(upto, l) - f);
+            out.keys = size * 128;
+            return true;
+        }
+        before += total;
+    }
+    out = Piece{a.B + index - before, 0, 1, 128};
+    return out.seq < a.T;
+}
+
 // ---- codes to operands --------------------------------------------------------------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -193,7 +264,13 @@ __device__ __forceinline__ Pages find_pages(const AttnArgs& a, const int32_t* bt
     return p;
 }
 
-template <int KIND, int D> __device__ __forceinline__ void load_step(const AttnArgs& a, const Pages& p, int h, int lane, Step<KIND, D>& s) {
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <bool ONCE, typename T> __device__ __forceinline__ T take(const uint8_t* p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+    else return *reinterpret_cast<const T*>(p);
+}
+template <int KIND, int D, bool ONCE> __device__ __forceinline__ void load_step(const AttnArgs& a, const Pages& p, int h, int lane, Step<KIND, D>& s) {
     constexpr int RB = row_bytes<KIND, D>();
     const int r = lane & 15, h4 = lane >> 4;
 #pragma unroll
@@ -203,17 +280,17 @@ template <int KIND, int D> __device__ __forceinline__ void load_step(const AttnA
         if constexpr (KIND == kInt8) {
 #pragma unroll
             for (int u = 0; u < D / 64; ++u) {
-                const uint4 x = *reinterpret_cast<const uint4*>(kp + 64 * u + 16 * h4);
+                const u32x4 x = take<ONCE, u32x4>(kp + 64 * u + 16 * h4);
                 s.k[g][4 * u] = x.x, s.k[g][4 * u + 1] = x.y, s.k[g][4 * u + 2] = x.z, s.k[g][4 * u + 3] = x.w;
             }
             s.ks[g] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(a.cache.ks) + row + 4 * h4);
             s.vs[g] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(a.cache.vs) + row + 4 * h4);
         } else {
             if constexpr (D == 128) {
-                const uint4 x = *reinterpret_cast<const uint4*>(kp + 16 * h4);
+                const u32x4 x = take<ONCE, u32x4>(kp + 16 * h4);
                 s.k[g][0] = x.x, s.k[g][1] = x.y, s.k[g][2] = x.z, s.k[g][3] = x.w;
             } else {
-                const uint2 x = *reinterpret_cast<const uint2*>(kp + 8 * h4);
+                const u32x2 x = take<ONCE, u32x2>(kp + 8 * h4);
                 s.k[g][0] = x.x, s.k[g][1] = x.y;
             }
             s.ke[g] = *(reinterpret_cast<const uint8_t*>(a.cache.ks) + (row + r) * (D / 32) + h4 * (D / 32) / 4);
@@ -230,12 +307,12 @@ template <int KIND, int D> __device__ __forceinline__ void load_step(const AttnA
         for (int i = 0; i < 4; ++i) {
             const uint8_t* vp = a.cache.v + (row + 4 * h4 + i) * RB + (RB / 16) * r;
             if constexpr (RB == 128) {
-                const uint2 x = *reinterpret_cast<const uint2*>(vp);
+                const u32x2 x = take<ONCE, u32x2>(vp);
                 s.v[4 * g + i][0] = x.x, s.v[4 * g + i][1] = x.y;
             } else if constexpr (RB == 64) {
-                s.v[4 * g + i][0] = *reinterpret_cast<const uint32_t*>(vp);
+                s.v[4 * g + i][0] = take<ONCE, uint32_t>(vp);
             } else {
-                s.v[4 * g + i][0] = *reinterpret_cast<const uint16_t*>(vp);
+                s.v[4 * g + i][0] = take<ONCE, uint16_t>(vp);
             }
         }
     }
@@ -308,7 +385,8 @@ template <int KIND> __device__ __forceinline__ uint32_t round2(float a, float b)
 
 // ---- the tile -----------------------------------------------------------------------------------------------------------------------------------------
 // GROUPS: the items are groups of sequences, the keys those that each shares; otherwise sequences, their keys behind what they share.
-template <int KIND, int D, int NQT, bool GROUPS>
+// ONCE: the codes are marked as read once.
+template <int KIND, int D, int NQT, bool GROUPS, bool ONCE>
 __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_rows_kernel(const AttnArgs a) {
     constexpr int ROWS = 16 * NQT, NC = D / 32, ND = D / 16;
     __shared__ __attribute__((aligned(16))) f32x4 so[3][ND][64];
@@ -316,10 +394,27 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, h4 = lane >> 4;
     const int heads = a.cache.heads, G = a.hq / heads;
-    const int h = blockIdx.x % heads, split = blockIdx.y;
+    const int h = blockIdx.x % heads;
+    int split = blockIdx.y;
     Tile tile;
-    if (!find_tile<GROUPS>(a, blockIdx.x / heads, G, ROWS, lane, tile)) return;
+    Piece own{0, 0, 0, 0};
+    if (!GROUPS && a.share) {
+        if (!find_piece(a, blockIdx.x / heads, lane, own)) return;
+        tile = Tile{min(own.seq, a.B), own.seq, 1, 0};
+        split = own.split;
+        if (split == 0)   // the slots that its rows have no pieces for
+            for (int i = threadIdx.x; i < G * (a.slots - own.splits); i += 256)
+                a.part_ml[(int64_t)(own.splits + i / G) * a.T * a.hq + (int64_t)own.seq * a.hq + h * G + i % G] = float2{-INFINITY, 0.f};
+    } else if (!find_tile<GROUPS>(a, blockIdx.x / heads, G, ROWS, lane, tile)) {
+        return;
+    }
 
+    tile.same();
+    split = __builtin_amdgcn_readfirstlane(split);
+    // keys from the first on, if no piece is cut: the wave's first pages do not wait for the context's length
+    Pages early{{-1, -1}, {0, 0}};
+    const bool guess = !GROUPS && !a.share && a.splits == 1 && !a.group_start && tile.item < a.B;
+    if (guess) early = find_pages(a, a.bt + (int64_t)tile.item * a.bt_stride, w * 32, a.width * a.cache.page);
     // the rows of this lane: the last position each sees, and its queries
     const Item<GROUPS> item(a, tile, lane);
     if (split == 0) item.mark(a, tile, ROWS, h, G, 256);
@@ -332,7 +427,7 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
         const bool valid = R < tile.toks * G;
         const int t = tile.tok0 + (valid ? R / G : 0), hd = h * G + R % G;
         rpos[qt] = valid ? item.sees(a, tile, t) : -1;
-        last = max(last, rpos[qt]);
+        if constexpr (GROUPS) last = max(last, rpos[qt]);
         const uint16_t* qp = a.q + t * a.q_stride + (int64_t)hd * D;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -341,13 +436,21 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
             qf[qt][c] = v;
         }
     }
+    if constexpr (GROUPS) {
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) last = max(last, __shfl_xor(last, o, 64));
-    last = __builtin_amdgcn_readfirstlane(last);
+        for (int o = 1; o < 16; o <<= 1) last = max(last, __shfl_xor(last, o, 64));
+        last = __builtin_amdgcn_readfirstlane(last);
+    } else {   // the tile's last token's
+        last = __builtin_amdgcn_readfirstlane(item.ctx - tile.toks + min(tile.toks - 1, (tile.at + ROWS - 1) / G));
+    }
     int ks, ke;
-    item.piece(a, tile, last, split, 128, ks, ke);
+    if (!GROUPS && a.share) {
+        ks = split * own.keys;
+        ke = min(last + 1, ks + own.keys);
+    } else {
+        item.piece(a, tile, last, split, 128, ks, ke);
+    }
     const int32_t* bt = a.bt + (int64_t)item.seq * a.bt_stride;
-
     float m[NQT], l[NQT];
     f32x4 o[NQT][ND];
 #pragma unroll
@@ -446,10 +549,11 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
 
     {
         int t0 = ks + w * 32;
-        Pages pg = find_pages(a, bt, t0, ke);
+        Pages pg = early;
+        if (!guess) pg = find_pages(a, bt, t0, ke);
         for (; t0 < ke; t0 += 128) {
             Step<KIND, D> s;
-            load_step<KIND, D>(a, pg, h, lane, s);
+            load_step<KIND, D, ONCE>(a, pg, h, lane, s);
             const Pages next = find_pages(a, bt, t0 + 128, ke);
             compute(t0, pg, s);
             pg = next;
@@ -670,8 +774,28 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
     const int h = blockIdx.x % heads, split = blockIdx.y;
     Tile tile;
     if (!find_tile<GROUPS>(a, blockIdx.x / heads, G, ROWS, lane, tile)) return;
+    tile.same();
     const Item<GROUPS> item(a, tile, lane);
     if (split == 0) item.mark(a, tile, ROWS, h, G, 64 * WAVES);
+
+    // The keys come first: nothing of the rows is needed to fetch them.  A group's rows see all that it shares, unless a context ends in it: then some are masked.
+    int ks, ke;
+    item.piece(a, tile, GROUPS ? INT_MAX - 1 : item.ctx - tile.toks + min(tile.toks - 1, (tile.at + ROWS - 1) / G), split, KT, ks, ke);
+    ks = __builtin_amdgcn_readfirstlane(ks);
+    ke = __builtin_amdgcn_readfirstlane(ke);
+    const int32_t* bt = a.bt + (int64_t)item.seq * a.bt_stride;
+    const bool of_keys = w < WAVES / 2;
+    const int part = of_keys ? w : w - WAVES / 2;   // of the step's keys
+    Fetch<KIND, D> f;
+    auto fetch = [&](int at) {
+        if (of_keys) f.keys(a, bt, at + 32 * part, ke, h, lane);
+        else f.values(a, bt, at + 32 * part, ke, h, lane);
+    };
+    auto store = [&](TS& s) {
+        if (of_keys) f.template put_keys<WAVES>(s, part, ke, a.scale_log2, lane);
+        else f.template put_values<WAVES>(s, part, lane);
+    };
+    if (ks < ke) fetch(ks);
 
     const int R = tile.at + 32 * w + r, live_rows = tile.toks * G;
     const bool valid = R < live_rows;
@@ -694,20 +818,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
     }
     first = __builtin_amdgcn_readfirstlane(first);
     last = __builtin_amdgcn_readfirstlane(last);
-    int all;   // the last that any row of the tile sees
-    {
-        int* seen = reinterpret_cast<int*>(lds);
-        if (lane == 0) seen[w] = last;
-        __syncthreads();
-        all = seen[0];
-#pragma unroll
-        for (int i = 1; i < WAVES; ++i) all = max(all, seen[i]);
-        all = __builtin_amdgcn_readfirstlane(all);
-        __syncthreads();
-    }
-    int ks, ke;
-    item.piece(a, tile, all, split, KT, ks, ke);
-    const int32_t* bt = a.bt + (int64_t)item.seq * a.bt_stride;
 
     // int8: value scales so far are up to `unit`, and sums are held 2^lift = 64 / unit times as large: probabilities, up to 2^8, times scales fit float16
     float m = -INFINITY, l = 0.f, unit = KIND == kInt8 ? 0x1p-100f : 0.f, lift = 0.f;
@@ -716,18 +826,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
     for (int T = 0; T < NT; ++T)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[T][i] = 0.f;
-
-    const bool of_keys = w < WAVES / 2;
-    const int part = of_keys ? w : w - WAVES / 2;   // of the step's keys
-    Fetch<KIND, D> f;
-    auto fetch = [&](int at) {
-        if (of_keys) f.keys(a, bt, at + 32 * part, ke, h, lane);
-        else f.values(a, bt, at + 32 * part, ke, h, lane);
-    };
-    auto store = [&](TS& s) {
-        if (of_keys) f.template put_keys<WAVES>(s, part, ke, a.scale_log2, lane);
-        else f.template put_values<WAVES>(s, part, lane);
-    };
 
     auto scores = [&](const TS& s, int sub) {
         f32x16 sc;
@@ -809,7 +907,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
     };
 
     if (ks < ke) {
-        fetch(ks);
         store(steps[0]);
         __syncthreads();
         int b = 0;
@@ -898,8 +995,10 @@ __global__ void __launch_bounds__(256) quant_join_kernel(const float* __restrict
         for (int k = 1; k < L; k <<= 1) sum += __shfl_xor(sum, k, L);
         l += sum;
         const float* p = part_o + (s0 * rows + row) * D + 4 * c;
+        const uint64_t used = __ballot(there) >> (threadIdx.x & 63 & ~(L - 1)) & ((1ull << L) - 1);
+        const int upto = n <= 8 ? n : used ? 64 - __builtin_clzll(used) : 0;   // behind the last that there is nothing is read; a few do not wait to be known
 #pragma unroll 4
-        for (int i = 0; i < n; ++i, p += per * rows * D) {
+        for (int i = 0; i < upto; ++i, p += per * rows * D) {
             const f32x4 x = *reinterpret_cast<const f32x4*>(p);
             const float f = __shfl(w, i, L);
             const bool on = __shfl((int)there, i, L);   // what an empty piece has there was never written
@@ -928,11 +1027,13 @@ __global__ void __launch_bounds__(256) quant_join_kernel(const float* __restrict
 }
 
 template <int KIND, int D, bool GROUPS> void launch_rows(int rows, const AttnArgs& a, int64_t tiles, hipStream_t st) {
+    const bool once = (int64_t)a.B * a.width * a.cache.page * a.cache.heads * row_bytes<KIND, D>() * 2 >= (int64_t)192 << 20;
     const dim3 g((unsigned)(tiles * a.cache.heads), a.splits), b(256);
     if (rows == 16) {
-        hipLaunchKernelGGL((quant_rows_kernel<KIND, D, 1, GROUPS>), g, b, 0, st, a);
+        if (!GROUPS && once) hipLaunchKernelGGL((quant_rows_kernel<KIND, D, 1, GROUPS, !GROUPS>), g, b, 0, st, a);
+        else hipLaunchKernelGGL((quant_rows_kernel<KIND, D, 1, GROUPS, false>), g, b, 0, st, a);
     } else if (rows == 32) {
-        hipLaunchKernelGGL((quant_rows_kernel<KIND, D, 2, GROUPS>), g, b, 0, st, a);
+        hipLaunchKernelGGL((quant_rows_kernel<KIND, D, 2, GROUPS, false>), g, b, 0, st, a);
     } else if (rows == 128) {
         constexpr int lds = 2 * sizeof(TileStep<KIND, D, 4>);
         lds_limit<quant_tile_kernel<KIND, D, 4, GROUPS>>(lds);
@@ -950,25 +1051,23 @@ template <bool GROUPS> void launch_rows_of(int kind, int D, int rows, const Attn
     else launch_rows<kFp4, 128, GROUPS>(rows, a, tiles, st);
 }
 
-// Rows of a tile, by the rows that an item has on average
-int tile_of(int64_t rows, int64_t items) {
+// Rows of a tile, by the rows that an item has on average, and the keys
+int tile_of(int64_t rows, int64_t items, int64_t keys) {
     const int64_t per = items > 0 ? rows / items : rows;
-    const int k = knob("qrows", 0);
-    if (k && per > 32) return k;
-    return per <= 16 ? 16 : per <= 32 ? 32 : per <= 128 ? 128 : 256;
+    return per <= 16 ? 16 : per <= 32 ? 32 : per <= 128 || keys < 2048 ? 128 : 256;
 }
 
 }  // namespace
 
 // What a call needs beside its tensors: rows of tiles, pieces of the keys.  keys: at most so many an item, by the table's width.
-AttnPlan quant_attention_plan(int T, int B, int groups, int hq, int heads, int64_t keys) {
+AttnPlan quant_attention_plan(int T, int B, bool single, int groups, int hq, int heads, int64_t keys) {
     AttnPlan p{};
     const int64_t rows = (int64_t)T * (hq / heads);
     auto side = [&](int64_t items, int& tile, int64_t& tiles, int& splits) {
-        tile = tile_of(rows, items);
+        tile = tile_of(rows, items, keys);
         tiles = rows / tile + items + 1;
         const int64_t wgs = ((rows + tile - 1) / tile > items ? (rows + tile - 1) / tile : items) * heads;
-        const int64_t target = tile <= 32 ? knob("qat", 1024) : tile == 128 ? knob("qtt", 512) : knob("qtt", 512) / 2, least = tile <= 32 ? 256 : tile;
+        const int64_t target = tile <= 32 ? 1024 : 256, least = tile <= 32 ? 256 : tile / 2;
         int64_t s = tile <= 32 ? (target + wgs - 1) / wgs : (target + wgs / 2) / wgs;
         s = s < (keys + least - 1) / least ? s : (keys + least - 1) / least;
         splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
@@ -976,6 +1075,12 @@ AttnPlan quant_attention_plan(int T, int B, int groups, int hq, int heads, int64
     side(B, p.own_rows, p.own_tiles, p.own_splits);
     if (groups > 0) side(groups, p.group_rows, p.group_tiles, p.group_splits);
     p.slots = p.own_splits + p.group_splits;
+    // few sequences of one token each, whose lengths decide how long the card is busy: pieces of one size
+    if (single && groups == 0 && B >= 16 && B <= 256 && p.own_rows >= hq / heads && p.own_splits > 1) {
+        p.share = (int)((1024 + heads - 1) / heads);
+        p.slots = p.own_splits * 4 < 64 ? p.own_splits * 4 : 64;
+        p.own_tiles = p.share + B + (T - B);
+    }
     return p;
 }
 
@@ -985,16 +1090,17 @@ void launch_quant_attention(int kind, int D, const AttnPlan& p, const uint16_t* 
     if (T == 0) return;
     AttnArgs a{q, q_stride, cache, bt, bt_stride, width, q_start, ctx_len, groups ? group_start : nullptr, prefix_len, B, T, groups, hq, scale * 1.4426950408889634f,
                out, part_o, reinterpret_cast<float2*>(part_ml), p.slots, 0, 0,
-               (cache.page & (cache.page - 1)) ? -1 : __builtin_ctz(cache.page)};
+               (cache.page & (cache.page - 1)) ? -1 : __builtin_ctz(cache.page), 0};
     if (groups) {
         a.splits = p.group_splits;
         a.slot0 = 0;
         launch_rows_of<true>(kind, D, p.group_rows, a, p.group_tiles, st);
     }
-    a.splits = p.own_splits;
+    a.splits = p.share ? 1 : p.own_splits;
+    a.share = p.share;
     a.slot0 = p.group_splits;
     // one token of each sequence: tiles are counted without a look at where sequences begin
-    const int64_t tiles = q_start ? p.own_tiles : (int64_t)T * ((hq / cache.heads + p.own_rows - 1) / p.own_rows);
+    const int64_t tiles = q_start || p.share ? p.own_tiles : (int64_t)T * ((hq / cache.heads + p.own_rows - 1) / p.own_rows);
     launch_rows_of<false>(kind, D, p.own_rows, a, tiles, st);
     if (p.slots > 1) {
         const int64_t rows = (int64_t)T * hq;
