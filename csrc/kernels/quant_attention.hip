@@ -246,23 +246,23 @@ template <int KIND, int D> struct Step {   // 32 keys of one wave
     uint32_t k[2][KW], v[8][VW];
     f32x4 ks[2], vs[2];      // int8: scales of keys 16 g + 4 h4 + i
     uint32_t ke[2], ve[8];   // mxfp4: E of the lane's key and block; words of all blocks' E of its eight keys
+    int blk[2];              // pages, -1: not there
 };
-struct Pages {   // of a step's two halves; -1: not there
-    int blk[2], off[2];
-};
-
-__device__ __forceinline__ Pages find_pages(const AttnArgs& a, const int32_t* bt, int t0, int end) {
-    Pages p;
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-        const int at = t0 + 16 * g;
-        const int i = a.page_shift >= 0 ? at >> a.page_shift : at / a.cache.page;
-        const int blk = at < end ? __builtin_amdgcn_readfirstlane(bt[i]) : -1;
-        p.blk[g] = blk < a.cache.pages ? blk : -1;
-        p.off[g] = at - i * a.cache.page;
+// Pages of 32 keys' two halves: asked for a step ahead, known when they are used (the wait for them is then over)
+struct Pages {
+    int raw;   // of the first half in the lower lanes, of the second in the upper ones
+    __device__ __forceinline__ void ask(const AttnArgs& a, const int32_t* bt, int t0, int end, int lane) {
+        const int at = t0 + (lane >> 5) * 16;
+        raw = -1;
+        if (at < end) raw = bt[a.page_shift >= 0 ? at >> a.page_shift : at / a.cache.page];
     }
-    return p;
-}
+    // the page, -1: not there; its row
+    __device__ __forceinline__ int blk(const AttnArgs& a, int g) const {
+        const int b = __builtin_amdgcn_readlane(raw, 32 * g);
+        return b < a.cache.pages ? max(b, -1) : -1;
+    }
+    static __device__ __forceinline__ int off(const AttnArgs& a, int at) { return a.page_shift >= 0 ? at & (a.cache.page - 1) : at % a.cache.page; }
+};
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -270,12 +270,13 @@ template <bool ONCE, typename T> __device__ __forceinline__ T take(const uint8_t
     if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
     else return *reinterpret_cast<const T*>(p);
 }
-template <int KIND, int D, bool ONCE> __device__ __forceinline__ void load_step(const AttnArgs& a, const Pages& p, int h, int lane, Step<KIND, D>& s) {
+template <int KIND, int D, bool ONCE> __device__ __forceinline__ void load_step(const AttnArgs& a, const Pages& p, int t0, int h, int lane, Step<KIND, D>& s) {
     constexpr int RB = row_bytes<KIND, D>();
     const int r = lane & 15, h4 = lane >> 4;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-        const int64_t row = ((int64_t)max(p.blk[g], 0) * a.cache.heads + h) * a.cache.page + p.off[g];   // of 16, all of one page
+        s.blk[g] = p.blk(a, g);
+        const int64_t row = ((int64_t)max(s.blk[g], 0) * a.cache.heads + h) * a.cache.page + Pages::off(a, t0 + 16 * g);   // of 16, all of one page
         const uint8_t* kp = a.cache.k + (row + r) * RB;
         if constexpr (KIND == kInt8) {
 #pragma unroll
@@ -347,35 +348,48 @@ __device__ __forceinline__ uint32_t pair8(uint32_t first, uint32_t second, int i
     const f16x2 x = __builtin_bit_cast(f16x2, u);
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x, f16x2{(_Float16)32768.f, (_Float16)32768.f}, f16x2{(_Float16)-0.25f, (_Float16)-0.25f}));
 }
+// Two operands of V at a time, of neighbouring dimensions 2 k and 2 k + 1 of the lane's D / 16: eight 16-bit numbers each
 template <int KIND, int D> struct Values {
-    uint32_t w[D / 16][4];   // operand dt: eight 16-bit numbers
-    __device__ __forceinline__ void make(Step<KIND, D>& s, int r) {
+    const uint32_t (&v)[8][Step<KIND, D>::VW];   // int8: with the codes' top bits turned
+    float scale[8];                              // mxfp4
+    __device__ __forceinline__ Values(Step<KIND, D>& s, int r) : v(s.v) {
         if constexpr (KIND == kInt8) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
 #pragma unroll
                 for (int x = 0; x < Step<KIND, D>::VW; ++x) s.v[j][x] ^= 0x80808080u;
-#pragma unroll
-            for (int dt = 0; dt < D / 16; ++dt)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[dt][j] = pair8(s.v[2 * j][dt >> 2], s.v[2 * j + 1][dt >> 2], dt & 3);
         } else {
             const int sh = 8 * (r * (D / 16) / 32);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                bf16x2 a[4], b[4];
-                codes4(s.v[2 * j][0], __uint_as_float(((s.ve[2 * j] >> sh) & 255) << 23), a);
-                codes4(s.v[2 * j + 1][0], __uint_as_float(((s.ve[2 * j + 1] >> sh) & 255) << 23), b);
-#pragma unroll
-                for (int dt = 0; dt < D / 16; ++dt)
-                    w[dt][j] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b[dt >> 1]), __builtin_bit_cast(uint32_t, a[dt >> 1]), dt & 1 ? 0x07060302u : 0x05040100u);
-            }
+            for (int j = 0; j < 8; ++j) scale[j] = __uint_as_float(((s.ve[j] >> sh) & 255) << 23);
         }
     }
-    __device__ __forceinline__ f32x4 mul(int dt, const uint32_t (&p)[4], f32x4 acc) const {
-        const uint4 x{w[dt][0], w[dt][1], w[dt][2], w[dt][3]}, y{p[0], p[1], p[2], p[3]};
-        if constexpr (KIND == kInt8) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), acc, 0, 0, 0);
-        else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), acc, 0, 0, 0);
+    __device__ __forceinline__ uint32_t two(int j, int k) const {   // bfloat16 of codes 2 k and 2 k + 1
+        const uint32_t w = v[j][0];
+        return __builtin_bit_cast(uint32_t, k == 0   ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale[j], 0)
+                                            : k == 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale[j], 1)
+                                            : k == 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale[j], 2)
+                                                     : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale[j], 3));
+    }
+    __device__ __forceinline__ void pair(int k, uint4 (&o)[2]) const {
+        uint32_t w[2][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (KIND == kInt8) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) w[e][j] = pair8(v[2 * j][(2 * k + e) >> 2], v[2 * j + 1][(2 * k + e) >> 2], (2 * k + e) & 3);
+            } else {
+                const uint32_t a = two(2 * j, k), b = two(2 * j + 1, k);
+                w[0][j] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+                w[1][j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            }
+        }
+        o[0] = uint4{w[0][0], w[0][1], w[0][2], w[0][3]};
+        o[1] = uint4{w[1][0], w[1][1], w[1][2], w[1][3]};
+    }
+    static __device__ __forceinline__ f32x4 mul(const uint4& v, const uint4& p, f32x4 acc) {
+        if constexpr (KIND == kInt8) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, v), __builtin_bit_cast(f16x8, p), acc, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, p), acc, 0, 0, 0);
     }
 };
 template <int KIND> __device__ __forceinline__ uint32_t round2(float a, float b) {
@@ -412,9 +426,9 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
     tile.same();
     split = __builtin_amdgcn_readfirstlane(split);
     // keys from the first on, if no piece is cut: the wave's first pages do not wait for the context's length
-    Pages early{{-1, -1}, {0, 0}};
+    Pages pg{-1};
     const bool guess = !GROUPS && !a.share && a.splits == 1 && !a.group_start && tile.item < a.B;
-    if (guess) early = find_pages(a, a.bt + (int64_t)tile.item * a.bt_stride, w * 32, a.width * a.cache.page);
+    if (guess) pg.ask(a, a.bt + (int64_t)tile.item * a.bt_stride, w * 32, a.width * a.cache.page, lane);
     // the rows of this lane: the last position each sees, and its queries
     const Item<GROUPS> item(a, tile, lane);
     if (split == 0) item.mark(a, tile, ROWS, h, G, 256);
@@ -461,8 +475,8 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
         for (int dt = 0; dt < ND; ++dt) o[qt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    float unit = 0x1p-100f;   // int8: probabilities times value scales are held in float16 as 2^14 / unit of themselves; no scale so far is over it
-    auto compute = [&](int t0, const Pages& pg, Step<KIND, D>& s) {
+    float unit = 0x1p-100f, lift = 0.f;   // int8: value scales so far are up to `unit`; sums are held 2^lift = 2^14 / unit times as large, so probabilities times scales fit float16
+    auto compute = [&](int t0, Step<KIND, D>& s) {
         f32x4 sc[NQT][2];
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
@@ -492,28 +506,23 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
             }
         }
         bool there[8];   // keys of this lane: there, and before the end
-        float kmul[8], vmul[8];
+        float kmul[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            there[j] = pg.blk[j >> 2] >= 0 && t0 + 16 * (j >> 2) + 4 * h4 + (j & 3) < ke;
+            there[j] = s.blk[j >> 2] >= 0 && t0 + 16 * (j >> 2) + 4 * h4 + (j & 3) < ke;
             kmul[j] = KIND == kInt8 ? s.ks[j >> 2][j & 3] * a.scale_log2 : a.scale_log2;
         }
-        float grown = 1.f;
+        const float was = lift;
         if constexpr (KIND == kInt8) {
             float top = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = fmaxf(top, there[j] ? s.vs[j >> 2][j & 3] : 0.f);
             if (__ballot(top > unit)) {
-                top = 2.f * rows_max(top);
-                grown = unit / top;
-                unit = top;
+                unit = 2.f * rows_max(top);
+                lift = __log2f(16384.f / unit);
             }
-            const float up = 16384.f / unit;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) vmul[j] = s.vs[j >> 2][j & 3] * up;
         }
-        Values<KIND, D> val;
-        val.make(s, r);
+        uint4 pw[NQT];
 #pragma unroll
         for (int qt = 0; qt < NQT; ++qt) {
             float mx = -INFINITY;
@@ -526,8 +535,8 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
                 mx = fmaxf(mx, v);
             }
             mx = fmaxf(m[qt], rows_max(mx));
-            const float base = mx == -INFINITY ? 0.f : mx;
-            const float alpha = __builtin_amdgcn_exp2f(m[qt] - base);
+            const float base = mx == -INFINITY ? 0.f : mx - lift;
+            const float alpha = __builtin_amdgcn_exp2f(m[qt] - was - base);
             m[qt] = mx;
             float ps = 0.f, p[8];
 #pragma unroll
@@ -537,35 +546,38 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
                     if (nan >> j & 1) p[j] = seen[j] ? __builtin_nanf("") : 0.f;
                 }
                 ps += p[j];
-                if constexpr (KIND == kInt8) p[j] = seen[j] ? p[j] * vmul[j] : 0.f;
+                if constexpr (KIND == kInt8) p[j] = seen[j] ? p[j] * s.vs[j >> 2][j & 3] : 0.f;
             }
             l[qt] = l[qt] * alpha + ps;
-            const uint32_t pw[4] = {round2<KIND>(p[0], p[1]), round2<KIND>(p[2], p[3]), round2<KIND>(p[4], p[5]), round2<KIND>(p[6], p[7])};
-            const float old = alpha * grown;
+            pw[qt] = uint4{round2<KIND>(p[0], p[1]), round2<KIND>(p[2], p[3]), round2<KIND>(p[4], p[5]), round2<KIND>(p[6], p[7])};
 #pragma unroll
-            for (int dt = 0; dt < ND; ++dt) o[qt][dt] = val.mul(dt, pw, o[qt][dt] * old);
+            for (int dt = 0; dt < ND; ++dt) o[qt][dt] *= alpha;
+        }
+        const Values<KIND, D> val(s, r);
+#pragma unroll
+        for (int k = 0; k < ND / 2; ++k) {
+            uint4 v[2];
+            val.pair(k, v);
+#pragma unroll
+            for (int qt = 0; qt < NQT; ++qt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) o[qt][2 * k + e] = val.mul(v[e], pw[qt], o[qt][2 * k + e]);
         }
     };
 
     {
         int t0 = ks + w * 32;
-        Pages pg = early;
-        if (!guess) pg = find_pages(a, bt, t0, ke);
+        if (!guess) pg.ask(a, bt, t0, ke, lane);
         for (; t0 < ke; t0 += 128) {
             Step<KIND, D> s;
-            load_step<KIND, D, ONCE>(a, pg, h, lane, s);
-            const Pages next = find_pages(a, bt, t0 + 128, ke);
-            compute(t0, pg, s);
-            pg = next;
+            load_step<KIND, D, ONCE>(a, pg, t0, h, lane, s);
+            pg.ask(a, bt, t0 + 128, ke, lane);
+            compute(t0, s);
         }
     }
-    if constexpr (KIND == kInt8) {
-        const float f = unit * (1.f / (16384.f * kCodeUnit));
 #pragma unroll
-        for (int qt = 0; qt < NQT; ++qt)
-#pragma unroll
-            for (int dt = 0; dt < ND; ++dt) o[qt][dt] *= f;
-    }
+    for (int qt = 0; qt < NQT; ++qt) m[qt] -= lift;
+    constexpr float kMul = KIND == kInt8 ? 1.f / kCodeUnit : 1.f;
 
     // ---- the waves' sums: those of 16 rows to the wave that has them to write ----------------------------------------------------------------------------
 #pragma unroll
@@ -600,7 +612,7 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
             const bool live = R < tile.toks * G;
             const int64_t row = (int64_t)(tile.tok0 + R / G) * a.hq + h * G + R % G;
             if (live && a.slots == 1) {
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                const float inv = sum == 0.f ? 0.f : kMul / sum;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint16_t* dst = a.out + row * D + (4 * h4 + i) * ND;
@@ -619,7 +631,7 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
 #pragma unroll
                         for (int dt = 0; dt < ND; dt += 4)
                             *reinterpret_cast<f32x4*>(a.part_o + at * D + (4 * h4 + i) * ND + dt) =
-                                f32x4{o[qt][dt][i], o[qt][dt + 1][i], o[qt][dt + 2][i], o[qt][dt + 3][i]};
+                                f32x4{o[qt][dt][i], o[qt][dt + 1][i], o[qt][dt + 2][i], o[qt][dt + 3][i]} * kMul;
                 }
             }
         }
@@ -649,13 +661,14 @@ template <int KIND, int D> struct Fetch {
     uint32_t w[8 * VW > 4 * NP ? 8 * VW : 4 * NP];   // keys: 4 words of each piece; values: VW of each key
     uint32_t e[KIND == kFp4 ? 8 : 1];                // mxfp4: E of the pieces' blocks, or the words of the eight keys' values
     uint32_t scale;                                  // keys' waves, int8: lane i < 32: of key i, i >= 32: its value's; mxfp4: the word of key i's value
-    Pages pg;
-    int t0;
+    int blk[2], t0;
 
-    __device__ __forceinline__ int64_t row_of(const AttnArgs& a, int g, int h) const { return ((int64_t)max(pg.blk[g], 0) * a.cache.heads + h) * a.cache.page + pg.off[g]; }
-    __device__ __forceinline__ void keys(const AttnArgs& a, const int32_t* bt, int at, int end, int h, int lane) {
+    __device__ __forceinline__ int64_t row_of(const AttnArgs& a, int g, int h) const {
+        return ((int64_t)max(blk[g], 0) * a.cache.heads + h) * a.cache.page + Pages::off(a, t0 + 16 * g);
+    }
+    __device__ __forceinline__ void keys(const AttnArgs& a, const Pages& pg, int at, int h, int lane) {
         t0 = at;
-        pg = find_pages(a, bt, at, end);
+        blk[0] = pg.blk(a, 0), blk[1] = pg.blk(a, 1);
         const int64_t row0 = row_of(a, 0, h), row1 = row_of(a, 1, h);
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
@@ -672,9 +685,9 @@ template <int KIND, int D> struct Fetch {
         else if constexpr (D == 128) scale = reinterpret_cast<const uint32_t*>(a.cache.vs)[row];
         else scale = reinterpret_cast<const uint16_t*>(a.cache.vs)[row];
     }
-    __device__ __forceinline__ void values(const AttnArgs& a, const int32_t* bt, int at, int end, int h, int lane) {
+    __device__ __forceinline__ void values(const AttnArgs& a, const Pages& pg, int at, int h, int lane) {
         t0 = at;
-        pg = find_pages(a, bt, at, end);
+        blk[0] = pg.blk(a, 0), blk[1] = pg.blk(a, 1);
         const int r = lane & 15, h2 = lane >> 4 & 1;
         const int64_t row = (lane < 32 ? row_of(a, 0, h) : row_of(a, 1, h)) + 4 * h2;
 #pragma unroll
@@ -706,7 +719,7 @@ template <int KIND, int D> struct Fetch {
     // keys 32 i .. of the step
     template <int WAVES> __device__ __forceinline__ void put_keys(TileStep<KIND, D, WAVES>& s, int i, int end, float scale_log2, int lane) const {
         const uint32_t in = t0 >= end ? 0u : end - t0 >= 32 ? ~0u : (1u << (end - t0)) - 1u;
-        const uint32_t there = in & ((pg.blk[0] >= 0 ? 0xffffu : 0u) | (pg.blk[1] >= 0 ? 0xffff0000u : 0u));
+        const uint32_t there = in & ((blk[0] >= 0 ? 0xffffu : 0u) | (blk[1] >= 0 ? 0xffff0000u : 0u));
         const int key = lane & 31;
         const bool here = there >> key & 1;
         if constexpr (KIND == kInt8) {
@@ -754,11 +767,14 @@ template <int KIND, int D> struct Fetch {
                 st.ve[j] = (one > 252 ? 0 : one) << (8 * (r * (D / 16) / 32));
             }
         }
-        Values<KIND, D> val;
-        val.make(st, r);
+        const Values<KIND, D> val(st, r);
 #pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt)
-            *reinterpret_cast<uint4*>(s.v + (16 * dt + r) * s.VS + (4 * i + (lane >> 4)) * 16) = uint4{val.w[dt][0], val.w[dt][1], val.w[dt][2], val.w[dt][3]};
+        for (int k = 0; k < D / 32; ++k) {
+            uint4 o[2];
+            val.pair(k, o);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) *reinterpret_cast<uint4*>(s.v + (16 * (2 * k + x) + r) * s.VS + (4 * i + (lane >> 4)) * 16) = o[x];
+        }
     }
 };
 
@@ -787,9 +803,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
     const bool of_keys = w < WAVES / 2;
     const int part = of_keys ? w : w - WAVES / 2;   // of the step's keys
     Fetch<KIND, D> f;
-    auto fetch = [&](int at) {
-        if (of_keys) f.keys(a, bt, at + 32 * part, ke, h, lane);
-        else f.values(a, bt, at + 32 * part, ke, h, lane);
+    Pages pg;
+    pg.ask(a, bt, ks + 32 * part, ke, lane);
+    auto fetch = [&](int at) {   // the step's codes, and the next one's pages
+        if (of_keys) f.keys(a, pg, at + 32 * part, h, lane);
+        else f.values(a, pg, at + 32 * part, h, lane);
+        pg.ask(a, bt, at + KT + 32 * part, ke, lane);
     };
     auto store = [&](TS& s) {
         if (of_keys) f.template put_keys<WAVES>(s, part, ke, a.scale_log2, lane);
@@ -1027,7 +1046,7 @@ __global__ void __launch_bounds__(256) quant_join_kernel(const float* __restrict
 }
 
 template <int KIND, int D, bool GROUPS> void launch_rows(int rows, const AttnArgs& a, int64_t tiles, hipStream_t st) {
-    const bool once = (int64_t)a.B * a.width * a.cache.page * a.cache.heads * row_bytes<KIND, D>() * 2 >= (int64_t)192 << 20;
+    const bool once = !a.group_start && (int64_t)a.B * a.width * a.cache.page * a.cache.heads * row_bytes<KIND, D>() * 2 >= (int64_t)192 << 20;
     const dim3 g((unsigned)(tiles * a.cache.heads), a.splits), b(256);
     if (rows == 16) {
         if (!GROUPS && once) hipLaunchKernelGGL((quant_rows_kernel<KIND, D, 1, GROUPS, !GROUPS>), g, b, 0, st, a);
