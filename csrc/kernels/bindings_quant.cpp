@@ -160,7 +160,7 @@ Tensor quant_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
     Tensor po, pm;
     if (p.slots > 1) {
         po = at::empty({p.slots, T * hq, D}, q.options().dtype(at::kFloat));
-        pm = at::empty({p.slots, T * hq, 2}, q.options().dtype(at::kFloat));
+        pm = at::empty({p.slots, T * hq}, q.options().dtype(at::kFloat));
     }
     chronos::qkv::launch_quant_attention(c.kind, c.D, p, bf(x), x.stride(0), c.c, block_table.data_ptr<int32_t>(), block_table.stride(0), (int)block_table.size(1), qs, cp,
                                          gs, pl, (int)B, (int)T, (int)groups, (int)hq, (float)scale, bfm(out), p.slots > 1 ? po.data_ptr<float>() : nullptr,

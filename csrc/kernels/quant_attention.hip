@@ -11,8 +11,11 @@
 //   * V: the operand wants eight keys of one dimension, the page has the dimensions of one key.  Row m of product dt is dimension m D / 16 + dt: a lane then needs the
 //     same D / 16 neighbouring bytes of its eight keys, for all products, and no exchange between lanes.
 // int8: a key's scale multiplies its scores, a value's the probabilities.  These are then rounded to float16 (2^-12): in bfloat16 the largest probability of a row, 1 times a scale, would
-// be off by up to 2^-9 where without scales it is exact (.0025 of the output's size in place of .0017, of which its own rounding is .0016).  float16 has the range as they are held as a part of the largest
-// scale so far: down to 2^-38 of it.  mxfp4: the conversion takes the scale, probabilities are bfloat16.
+// be off by up to 2^-9 where without scales it is exact (.0025 of the output's size in place of .0017, of which its own rounding is .0016).  Each row's sums have a reference
+// that keeps its products in float16's range, the largest at 2^7 to 2^15, whatever the scales are; what is 2^-32 of the largest and less may get lost.  mxfp4: the conversion takes the scale, probabilities are bfloat16.
+//
+// The reference that a row's probabilities are 2^(score - ref) of only moves when a score is far over it (2^8; int8: as float16 allows): rescaling the sums costs as much as all
+// else that a step does to them, and while it stays no lane needs to know of another.
 //
 // What no sum may take: keys behind the position, behind the context, on pages that the table does not have (numbers outside 0 .. pages - 1 are left out): their
 // scores are -inf and their probabilities zero by selection, not by product; their values cannot be NaN either (a value scale of NaN acts on the probabilities of
@@ -40,7 +43,7 @@ struct AttnArgs {
     float scale_log2;
     uint16_t* out;            // [T, hq, D]
     float* part_o;            // [slots, T * hq, D]
-    float2* part_ml;          // [slots, T * hq]: maximum (base 2) and sum
+    float* part_l;            // [slots, T * hq]: base-2 logarithm of the sum of probabilities, -inf: no keys; part_o is what they average to
     int slots, splits, slot0;
     int page_shift;           // pages of a power of two tokens; -1: others
     int share;                // 0: every sequence's keys in `splits` pieces; else pieces of one size, about so many a key head (find_piece)
@@ -167,7 +170,7 @@ template <bool GROUPS> struct Item {
                 for (int i = threadIdx.x; i < rows * a.slot0; i += threads) {
                     const int R = tile.at + i % rows;
                     if (R < tile.toks * G)
-                        a.part_ml[(int64_t)(i / rows) * a.T * a.hq + (int64_t)(tile.tok0 + R / G) * a.hq + h * G + R % G] = float2{-INFINITY, 0.f};
+                        a.part_l[(int64_t)(i / rows) * a.T * a.hq + (int64_t)(tile.tok0 + R / G) * a.hq + h * G + R % G] = -INFINITY;
                 }
     }
 };
@@ -397,14 +400,25 @@ template <int KIND> __device__ __forceinline__ uint32_t round2(float a, float b)
     else return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
 }
 
+// A row's reference moves: to `up` over base, the highest score so far or (int8) what its probabilities times scales allow; never down, once there is one.  x are the
+// scores over base, and then over the new one; returns what sums so far are to be multiplied by.
+template <int N> __device__ __forceinline__ float moved_ref(float& ref, float base, float mx, float up, float (&x)[N]) {
+    const float to = ref == -INFINITY ? (mx == -INFINITY ? -INFINITY : base + up) : base + fmaxf(up, 0.f);
+    const float d = base - (to == -INFINITY ? 0.f : to), f = ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(d);
+    ref = to;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] += d;
+    return f;
+}
+
 // ---- the tile -----------------------------------------------------------------------------------------------------------------------------------------
 // GROUPS: the items are groups of sequences, the keys those that each shares; otherwise sequences, their keys behind what they share.
 // ONCE: the codes are marked as read once.
 template <int KIND, int D, int NQT, bool GROUPS, bool ONCE>
-__global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_rows_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(256, NQT == 1 ? (KIND == kInt8 && D == 128 ? 3 : 4) : 2) quant_rows_kernel(const AttnArgs a) {
     constexpr int ROWS = 16 * NQT, NC = D / 32, ND = D / 16;
     __shared__ __attribute__((aligned(16))) f32x4 so[3][ND][64];
-    __shared__ float sm[3][64], sl[3][64];
+    __shared__ float sl[3][64];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, h4 = lane >> 4;
     const int heads = a.cache.heads, G = a.hq / heads;
@@ -418,7 +432,7 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
         split = own.split;
         if (split == 0)   // the slots that its rows have no pieces for
             for (int i = threadIdx.x; i < G * (a.slots - own.splits); i += 256)
-                a.part_ml[(int64_t)(own.splits + i / G) * a.T * a.hq + (int64_t)own.seq * a.hq + h * G + i % G] = float2{-INFINITY, 0.f};
+                a.part_l[(int64_t)(own.splits + i / G) * a.T * a.hq + (int64_t)own.seq * a.hq + h * G + i % G] = -INFINITY;
     } else if (!find_tile<GROUPS>(a, blockIdx.x / heads, G, ROWS, lane, tile)) {
         return;
     }
@@ -434,14 +448,17 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
     if (split == 0) item.mark(a, tile, ROWS, h, G, 256);
     int rpos[NQT];
     bf16x8 qf[NQT][NC];
-    int last = -1;   // the last position that any row of the tile sees
+    int first = INT_MAX, last = -1;   // the last position that all rows of the tile see, and that any does
 #pragma unroll
     for (int qt = 0; qt < NQT; ++qt) {
         const int R = tile.at + 16 * qt + r;
         const bool valid = R < tile.toks * G;
         const int t = tile.tok0 + (valid ? R / G : 0), hd = h * G + R % G;
-        rpos[qt] = valid ? item.sees(a, tile, t) : -1;
-        if constexpr (GROUPS) last = max(last, rpos[qt]);
+        rpos[qt] = valid ? item.sees(a, tile, t) : INT_MAX;   // what the rows behind the tile's make is not written
+        if constexpr (GROUPS) {
+            last = max(last, valid ? rpos[qt] : -1);
+            first = min(first, rpos[qt]);
+        }
         const uint16_t* qp = a.q + t * a.q_stride + (int64_t)hd * D;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -452,9 +469,14 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
     }
     if constexpr (GROUPS) {
 #pragma unroll
-        for (int o = 1; o < 16; o <<= 1) last = max(last, __shfl_xor(last, o, 64));
+        for (int o = 1; o < 16; o <<= 1) {
+            first = min(first, __shfl_xor(first, o, 64));
+            last = max(last, __shfl_xor(last, o, 64));
+        }
+        first = __builtin_amdgcn_readfirstlane(first);
         last = __builtin_amdgcn_readfirstlane(last);
-    } else {   // the tile's last token's
+    } else {   // the tile's first token's, and its last's
+        first = __builtin_amdgcn_readfirstlane(item.ctx - tile.toks + tile.at / G);
         last = __builtin_amdgcn_readfirstlane(item.ctx - tile.toks + min(tile.toks - 1, (tile.at + ROWS - 1) / G));
     }
     int ks, ke;
@@ -465,17 +487,16 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
         item.piece(a, tile, last, split, 128, ks, ke);
     }
     const int32_t* bt = a.bt + (int64_t)item.seq * a.bt_stride;
-    float m[NQT], l[NQT];
+    float ref[NQT], l[NQT];   // sums are of 2^(score - ref)
     f32x4 o[NQT][ND];
 #pragma unroll
     for (int qt = 0; qt < NQT; ++qt) {
-        m[qt] = -INFINITY;
+        ref[qt] = -INFINITY;
         l[qt] = 0.f;
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt) o[qt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    float unit = 0x1p-100f, lift = 0.f;   // int8: value scales so far are up to `unit`; sums are held 2^lift = 2^14 / unit times as large, so probabilities times scales fit float16
     auto compute = [&](int t0, Step<KIND, D>& s) {
         f32x4 sc[NQT][2];
 #pragma unroll
@@ -489,12 +510,19 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
                 for (int qt = 0; qt < NQT; ++qt) sc[qt][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[qt][c], sc[qt][g], 0, 0, 0);
             }
         }
-        uint32_t nan = 0;   // mxfp4: keys of this lane whose values are NaN, bit 4 g + i
+        // Values that are NaN, by their scales: 4-bit ones from 253 on (192 and more does not come from numbers: looked for in all keys at once), float ones that are
+        // not finite (or negative).  They count as zeros and their keys' scores as NaN.
+        uint32_t nan = 0, top = 0;   // of this lane's keys, bit j; int8: the largest scale's bits
         if constexpr (KIND == kFp4) {
-            uint32_t big = 0;   // E of 192 and more does not come from numbers: looked for in all keys at once
 #pragma unroll
-            for (int j = 0; j < 8; ++j) big |= s.ve[j] & (s.ve[j] << 1);
-            if (__ballot((big & 0x80808080u) != 0)) {
+            for (int j = 0; j < 8; ++j) top |= s.ve[j] & (s.ve[j] << 1) & 0x80808080u;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(s.vs[j >> 2][j & 3]));
+        }
+        const bool odd = __ballot(KIND == kFp4 ? top != 0 : top >= 0x7f800000u) != 0;
+        if (odd) {
+            if constexpr (KIND == kFp4) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -503,55 +531,62 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
                             nan |= 1u << j;
                             s.ve[j] &= ~(255u << (8 * b));
                         }
+            } else {
+                top = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    uint32_t v = __float_as_uint(s.vs[j >> 2][j & 3]);
+                    if (v >= 0x7f800000u) nan |= 1u << j, v = 0;
+                    top = max(top, v);
+                    s.vs[j >> 2][j & 3] = __uint_as_float(v);
+                }
             }
         }
-        bool there[8];   // keys of this lane: there, and before the end
-        float kmul[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            there[j] = s.blk[j >> 2] >= 0 && t0 + 16 * (j >> 2) + 4 * h4 + (j & 3) < ke;
-            kmul[j] = KIND == kInt8 ? s.ks[j >> 2][j & 3] * a.scale_log2 : a.scale_log2;
-        }
-        const float was = lift;
-        if constexpr (KIND == kInt8) {
-            float top = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, there[j] ? s.vs[j >> 2][j & 3] : 0.f);
-            if (__ballot(top > unit)) {
-                unit = 2.f * rows_max(top);
-                lift = __log2f(16384.f / unit);
-            }
-        }
+        const bool part = odd || t0 + 32 > ke || t0 + 31 > first || s.blk[0] < 0 || s.blk[1] < 0;   // some row does not see some key
+        // scores over the reference may be so high: int8, times the lane's scales, as float16 holds
+        const float most = KIND == kInt8 ? fminf(15.f - __log2f(__uint_as_float(top)), 100.f) : 8.f;
         uint4 pw[NQT];
 #pragma unroll
         for (int qt = 0; qt < NQT; ++qt) {
-            float mx = -INFINITY;
-            bool seen[8];
+            const float base = ref[qt] == -INFINITY ? 0.f : ref[qt];
+            float x[8], mx = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                seen[j] = there[j] && t0 + 16 * (j >> 2) + 4 * h4 + (j & 3) <= rpos[qt];
-                const float v = seen[j] ? sc[qt][j >> 2][j & 3] * kmul[j] : -INFINITY;
-                sc[qt][j >> 2][j & 3] = v;
-                mx = fmaxf(mx, v);
+                const float mul = KIND == kInt8 ? s.ks[j >> 2][j & 3] * a.scale_log2 : a.scale_log2;
+                x[j] = __builtin_fmaf(sc[qt][j >> 2][j & 3], mul, -base);
             }
-            mx = fmaxf(m[qt], rows_max(mx));
-            const float base = mx == -INFINITY ? 0.f : mx - lift;
-            const float alpha = __builtin_amdgcn_exp2f(m[qt] - was - base);
-            m[qt] = mx;
-            float ps = 0.f, p[8];
+            if (part) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                p[j] = __builtin_amdgcn_exp2f(sc[qt][j >> 2][j & 3] - base);
-                if constexpr (KIND == kFp4) {
-                    if (nan >> j & 1) p[j] = seen[j] ? __builtin_nanf("") : 0.f;
+                for (int j = 0; j < 8; ++j) {
+                    const int key = t0 + 16 * (j >> 2) + 4 * h4 + (j & 3);
+                    const bool seen = s.blk[j >> 2] >= 0 && key < ke && key <= rpos[qt];
+                    x[j] = !seen ? -INFINITY : nan >> j & 1 ? __builtin_nanf("") : x[j];
                 }
-                ps += p[j];
-                if constexpr (KIND == kInt8) p[j] = seen[j] ? p[j] * s.vs[j >> 2][j & 3] : 0.f;
             }
-            l[qt] = l[qt] * alpha + ps;
-            pw[qt] = uint4{round2<KIND>(p[0], p[1]), round2<KIND>(p[2], p[3]), round2<KIND>(p[4], p[5]), round2<KIND>(p[6], p[7])};
 #pragma unroll
-            for (int dt = 0; dt < ND; ++dt) o[qt][dt] *= alpha;
+            for (int j = 0; j < 8; ++j) mx = fmaxf(mx, x[j]);
+            if (__builtin_expect(__ballot(mx > (ref[qt] == -INFINITY ? -INFINITY : most)) != 0, false)) {
+                mx = rows_max(mx);
+                float up = mx;
+                if constexpr (KIND == kInt8) {
+                    up = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) up = fmaxf(up, x[j] + __log2f(s.vs[j >> 2][j & 3]));
+                    up = fmaxf(rows_max(up) - 7.f, mx - 90.f);
+                }
+                const float f = moved_ref(ref[qt], base, mx, up, x);
+                l[qt] *= f;
+#pragma unroll
+                for (int dt = 0; dt < ND; ++dt) o[qt][dt] *= f;
+            }
+            float p[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                p[j] = __builtin_amdgcn_exp2f(x[j]);
+                l[qt] += p[j];
+                if constexpr (KIND == kInt8) p[j] *= s.vs[j >> 2][j & 3];
+            }
+            pw[qt] = uint4{round2<KIND>(p[0], p[1]), round2<KIND>(p[2], p[3]), round2<KIND>(p[4], p[5]), round2<KIND>(p[6], p[7])};
         }
         const Values<KIND, D> val(s, r);
 #pragma unroll
@@ -575,63 +610,61 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
             compute(t0, s);
         }
     }
-#pragma unroll
-    for (int qt = 0; qt < NQT; ++qt) m[qt] -= lift;
-    constexpr float kMul = KIND == kInt8 ? 1.f / kCodeUnit : 1.f;
-
-    // ---- the waves' sums: those of 16 rows to the wave that has them to write ----------------------------------------------------------------------------
+    // ---- the waves' averages: those of 16 rows to the wave that has them to write ------------------------------------------------------------------------
 #pragma unroll
     for (int qt = 0; qt < NQT; ++qt) {
-        l[qt] = rows_sum(l[qt]);
+        const float all = rows_sum(l[qt]), inv = all == 0.f ? 0.f : (KIND == kInt8 ? 1.f / kCodeUnit : 1.f) / all;
+        const float lse = all == 0.f ? -INFINITY : ref[qt] + __log2f(all);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) o[qt][dt] *= inv;
         const int owner = qt & 3;
         const int place = w < owner ? w : w - 1;
         if (qt) __syncthreads();
         if (w != owner) {
-            sm[place][lane] = m[qt];
-            sl[place][lane] = l[qt];
+            sl[place][lane] = lse;
 #pragma unroll
             for (int dt = 0; dt < ND; ++dt) so[place][dt][lane] = o[qt][dt];
         }
         __syncthreads();
         if (w == owner) {
-            float mx = m[qt];
+            float mx = lse;
 #pragma unroll
-            for (int p = 0; p < 3; ++p) mx = fmaxf(mx, sm[p][lane]);
+            for (int p = 0; p < 3; ++p) mx = fmaxf(mx, sl[p][lane]);
             const float base = mx == -INFINITY ? 0.f : mx;
-            float f = __builtin_amdgcn_exp2f(m[qt] - base), sum = l[qt] * f;
+            float f = __builtin_amdgcn_exp2f(lse - base), sum = f;
 #pragma unroll
             for (int dt = 0; dt < ND; ++dt) o[qt][dt] *= f;
 #pragma unroll
             for (int p = 0; p < 3; ++p) {
-                f = __builtin_amdgcn_exp2f(sm[p][lane] - base);
-                sum += sl[p][lane] * f;
+                f = __builtin_amdgcn_exp2f(sl[p][lane] - base);
+                sum += f;
 #pragma unroll
                 for (int dt = 0; dt < ND; ++dt) o[qt][dt] += so[p][dt][lane] * f;
             }
             const int R = tile.at + 16 * qt + r;
             const bool live = R < tile.toks * G;
             const int64_t row = (int64_t)(tile.tok0 + R / G) * a.hq + h * G + R % G;
+            const float one = sum == 0.f ? 0.f : 1.f / sum;
             if (live && a.slots == 1) {
-                const float inv = sum == 0.f ? 0.f : kMul / sum;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint16_t* dst = a.out + row * D + (4 * h4 + i) * ND;
                     uint16_t v[ND];
 #pragma unroll
-                    for (int dt = 0; dt < ND; ++dt) v[dt] = f2bf(o[qt][dt][i] * inv);
+                    for (int dt = 0; dt < ND; ++dt) v[dt] = f2bf(o[qt][dt][i] * one);
                     if constexpr (ND == 8) *reinterpret_cast<u16x8*>(dst) = u16x8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
                     else *reinterpret_cast<u16x4*>(dst) = u16x4{v[0], v[1], v[2], v[3]};
                 }
             } else if (live) {
                 const int64_t at = (int64_t)(a.slot0 + split) * a.T * a.hq + row;
-                if (h4 == 0) a.part_ml[at] = float2{mx, sum};
+                if (h4 == 0) a.part_l[at] = sum == 0.f ? -INFINITY : base + __log2f(sum);
                 if (sum != 0.f) {   // nothing there is not read either
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
                         for (int dt = 0; dt < ND; dt += 4)
                             *reinterpret_cast<f32x4*>(a.part_o + at * D + (4 * h4 + i) * ND + dt) =
-                                f32x4{o[qt][dt][i], o[qt][dt + 1][i], o[qt][dt + 2][i], o[qt][dt + 3][i]} * kMul;
+                                f32x4{o[qt][dt][i], o[qt][dt + 1][i], o[qt][dt + 2][i], o[qt][dt + 3][i]} * one;
                 }
             }
         }
@@ -644,14 +677,13 @@ __global__ void __launch_bounds__(256, NQT == 1 ? 4 : NQT == 2 ? 2 : 1) quant_ro
 // loaded a step earlier, into the buffer that is not being read; one barrier a step.  16 bytes behind every row keep its readers, 16 bytes a lane and a row
 // each, out of each other's banks.  v_mfma_f32_32x32x16: a lane has 16 of 32 keys of one row, and the probabilities are the second product's operand as they are, its values' keys in the same order
 // (4 h + (j & 3) + 8 (j >> 2) of 16).
-// The maximum that probabilities are taken from is only moved when a score is 2^8 over it: rescaling the sums would cost as much as all else that a step does to them.
 template <int KIND, int D, int WAVES> struct TileStep {
     static constexpr int KT = 16 * WAVES, KS = 2 * D + 16, VS = 2 * KT + 16;   // bytes from key to key, and from dimension to dimension
     alignas(16) uint8_t k[KT * KS];
     alignas(16) uint8_t v[D * VS];
     alignas(16) float km[KT], vm[KT];   // int8: scales of keys, times scale_log2, and values; 0 where a key is not there
     uint32_t there[KT / 32], nan[KT / 32];
-    float top[KT / 32];                 // int8: largest of vm
+    float top[KT / 32];                 // int8: base-2 logarithm of the largest of vm
 };
 
 // 32 keys' codes on their way into LDS, by one wave: keys or values
@@ -724,13 +756,13 @@ template <int KIND, int D> struct Fetch {
         const bool here = there >> key & 1;
         if constexpr (KIND == kInt8) {
             float x = here ? __uint_as_float(scale) : 0.f;
-            const bool bad = lane >= 32 && !(x < INFINITY);
+            const bool bad = lane >= 32 && !(x >= 0.f && x < INFINITY);
             if (bad) x = 0.f;
             if (lane < 32) s.km[32 * i + key] = x * scale_log2;
             else s.vm[32 * i + key] = x;
             const float top = wave_max(lane < 32 ? 0.f : x);
             const uint32_t nan = (uint32_t)(__ballot(bad) >> 32);
-            if (lane == 0) s.top[i] = top, s.there[i] = there, s.nan[i] = nan;
+            if (lane == 0) s.top[i] = __log2f(top), s.there[i] = there, s.nan[i] = nan;
         } else {
             bool bad = false;
 #pragma unroll
@@ -838,8 +870,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
     first = __builtin_amdgcn_readfirstlane(first);
     last = __builtin_amdgcn_readfirstlane(last);
 
-    // int8: value scales so far are up to `unit`, and sums are held 2^lift = 64 / unit times as large: probabilities, up to 2^8, times scales fit float16
-    float m = -INFINITY, l = 0.f, unit = KIND == kInt8 ? 0x1p-100f : 0.f, lift = 0.f;
+    float ref = -INFINITY, l = 0.f;   // sums are of 2^(score - ref)
     f32x16 o[NT];
 #pragma unroll
     for (int T = 0; T < NT; ++T)
@@ -858,7 +889,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
     // 32 keys from t0 on, the step's sub-th, whose scores are made; makes the next ones' beside the probabilities
     f32x16 sc;
     auto compute = [&](const TS& s, int sub, int t0) {
-        const float base = m == -INFINITY ? -lift : m - lift;
+        const float base = ref == -INFINITY ? 0.f : ref;
         float x[16], mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
@@ -878,22 +909,21 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[i]);
-        mx = lanes_xor32(mx, LaneMax{});
-        float top = 0.f;
-        if constexpr (KIND == kInt8) top = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(s.top[sub])));
-        if (__builtin_expect(__ballot(mx > (m == -INFINITY ? -INFINITY : lift + 8.f)) != 0 || top > unit, false)) {
-            const float to = mx > -INFINITY ? fmaxf(mx + base, m) : m, from = m - lift;
-            if (top > unit) {
-                unit = 2.f * top;
-                lift = __log2f(64.f / unit);
+        // scores over the reference may be so high: int8, times the largest scale, as float16 holds
+        const float most = KIND == kInt8 ? fminf(15.f - s.top[sub], 100.f) : 8.f;
+        if (__builtin_expect(__ballot(mx > (ref == -INFINITY ? -INFINITY : most)) != 0, false)) {
+            mx = lanes_xor32(mx, LaneMax{});
+            float up = mx;
+            if constexpr (KIND == kInt8) {
+                up = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) up = fmaxf(up, x[i] + __log2f(s.vm[32 * sub + 4 * h2 + (i & 3) + 8 * (i >> 2)]));
+                up = fmaxf(lanes_xor32(up, LaneMax{}) - 7.f, mx - 90.f);
             }
-            const float now = to == -INFINITY ? -lift : to - lift, old = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(from - now), d = base - now;
-            m = to;
-            l *= old;
+            const float f = moved_ref(ref, base, mx, up, x);
+            l *= f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] += d;
-#pragma unroll
-            for (int T = 0; T < NT; ++T) o[T] *= old;
+            for (int T = 0; T < NT; ++T) o[T] *= f;
         }
         if (sub + 1 < KT / 32) sc = scores(s, sub + 1);
 #pragma unroll
@@ -950,8 +980,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
     // dimension D / 16 (row % 16) + row / 16: a lane has D / 16 neighbouring dimensions at a time.
     l = lanes_xor32(l, LaneSum{});
     const bool direct = a.slots == 1;
-    const float mul = (KIND == kInt8 ? 1.f / kCodeUnit : 1.f) * (direct ? (l == 0.f ? 0.f : 1.f / l) : 1.f);
-    if (!direct && h2 == 0 && valid) a.part_ml[(int64_t)(a.slot0 + split) * a.T * a.hq + (int64_t)t * a.hq + h * G + R % G] = float2{m - lift, l};
+    const float mul = l == 0.f ? 0.f : (KIND == kInt8 ? 1.f / kCodeUnit : 1.f) / l;
+    if (!direct && h2 == 0 && valid) a.part_l[(int64_t)(a.slot0 + split) * a.T * a.hq + (int64_t)t * a.hq + h * G + R % G] = l == 0.f ? -INFINITY : ref + __log2f(l);
     constexpr int OS = D + 4;   // floats from row to row
     float* mine = reinterpret_cast<float*>(lds) + w * 16 * OS;
 #pragma unroll
@@ -984,35 +1014,34 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
     }
 }
 
-// Rows of the pieces' sums: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  D / 4 lanes have a row, `per` such groups share its pieces and are joined through
-// LDS.  The maxima and sums of up to D / 4 pieces are read at once, a lane each, and handed round; what the pieces hold does not wait for them.
+// Rows of the pieces' averages o_s, of sums 2^(l_s): out = sum_s 2^(l_s - m) o_s / sum_s 2^(l_s - m).  D / 4 lanes have a row, `per` such groups share its pieces and are
+// joined through LDS.  The sums of up to D / 4 pieces are read at once, a lane each, and handed round; what the pieces hold does not wait for them.
 template <int D>
-__global__ void __launch_bounds__(256) quant_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, uint16_t* __restrict__ out, int64_t rows,
+__global__ void __launch_bounds__(256) quant_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_l, uint16_t* __restrict__ out, int64_t rows,
                                                          int slots, int per) {
     constexpr int L = D / 4, GR = 256 / L;
     __shared__ f32x4 so[GR][L];
     __shared__ float sl[GR], sm[GR];
     const int c = threadIdx.x % L, gr = threadIdx.x / L;
     const int64_t at = (int64_t)blockIdx.x * (GR / per) + gr / per, row = at < rows ? at : rows - 1;
-    float mx = -INFINITY, l = 0.f;
+    float mx = -INFINITY, sum = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = gr % per; s0 < slots; s0 += per * L) {   // pieces s0, s0 + per, ..: lane c has the c-th
-        const int n = min(L, (slots - s0 + per - 1) / per), mine = s0 + per * c;
-        const float2 ml = c < n ? part_ml[mine * rows + row] : float2{-INFINITY, 0.f};
-        const bool there = ml.y != 0.f;
-        float top = there ? ml.x : -INFINITY;
+        const int n = min(L, (slots - s0 + per - 1) / per);
+        const float mine = c < n ? part_l[(int64_t)(s0 + per * c) * rows + row] : -INFINITY;
+        const bool there = !(mine == -INFINITY);
+        float top = mine;
 #pragma unroll
         for (int k = 1; k < L; k <<= 1) top = fmaxf(top, __shfl_xor(top, k, L));
         top = fmaxf(top, mx);
         const float base = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(mx - base);
         mx = top;
-        l *= old;
         o *= old;
-        const float w = there ? __builtin_amdgcn_exp2f(ml.x - base) : 0.f;
-        float sum = there ? ml.y * w : 0.f;
+        const float w = there ? __builtin_amdgcn_exp2f(mine - base) : 0.f;
+        float all = w;
 #pragma unroll
-        for (int k = 1; k < L; k <<= 1) sum += __shfl_xor(sum, k, L);
-        l += sum;
+        for (int k = 1; k < L; k <<= 1) all += __shfl_xor(all, k, L);
+        sum = sum * old + all;
         const float* p = part_o + (s0 * rows + row) * D + 4 * c;
         const uint64_t used = __ballot(there) >> (threadIdx.x & 63 & ~(L - 1)) & ((1ull << L) - 1);
         const int upto = n <= 8 ? n : used ? 64 - __builtin_clzll(used) : 0;   // behind the last that there is nothing is read; a few do not wait to be known
@@ -1027,21 +1056,21 @@ __global__ void __launch_bounds__(256) quant_join_kernel(const float* __restrict
     }
     if (per > 1) {
         so[gr][c] = o;
-        if (c == 0) sl[gr] = l, sm[gr] = mx;
+        if (c == 0) sl[gr] = sum, sm[gr] = mx;
         __syncthreads();
         if (gr % per) return;
         for (int i = 1; i < per; ++i) mx = fmaxf(mx, sm[gr + i]);
         const float base = mx == -INFINITY ? 0.f : mx;
-        l = 0.f;
+        sum = 0.f;
         o = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int i = 0; i < per; ++i) {
             const float f = __builtin_amdgcn_exp2f(sm[gr + i] - base);
             o += so[gr + i][c] * f;
-            l += sl[gr + i] * f;
+            sum += sl[gr + i] * f;
         }
     }
     if (at >= rows) return;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     *reinterpret_cast<u16x4*>(out + row * D + 4 * c) = u16x4{f2bf(o[0] * inv), f2bf(o[1] * inv), f2bf(o[2] * inv), f2bf(o[3] * inv)};
 }
 
@@ -1105,10 +1134,10 @@ AttnPlan quant_attention_plan(int T, int B, bool single, int groups, int hq, int
 
 void launch_quant_attention(int kind, int D, const AttnPlan& p, const uint16_t* q, int64_t q_stride, const Cache& cache, const int32_t* bt, int64_t bt_stride, int width,
                             const int32_t* q_start, const int32_t* ctx_len, const int32_t* group_start, const int32_t* prefix_len, int B, int T, int groups, int hq,
-                            float scale, uint16_t* out, float* part_o, float* part_ml, hipStream_t st) {
+                            float scale, uint16_t* out, float* part_o, float* part_l, hipStream_t st) {
     if (T == 0) return;
     AttnArgs a{q, q_stride, cache, bt, bt_stride, width, q_start, ctx_len, groups ? group_start : nullptr, prefix_len, B, T, groups, hq, scale * 1.4426950408889634f,
-               out, part_o, reinterpret_cast<float2*>(part_ml), p.slots, 0, 0,
+               out, part_o, part_l, p.slots, 0, 0,
                (cache.page & (cache.page - 1)) ? -1 : __builtin_ctz(cache.page), 0};
     if (groups) {
         a.splits = p.group_splits;
@@ -1127,8 +1156,8 @@ void launch_quant_attention(int kind, int D, const AttnPlan& p, const uint16_t* 
         int per = 1;   // lanes' groups of a row: the rows fill the card with one, or there are pieces to share
         while (per < gr && per * 2 <= p.slots && rows * per < 2048 * gr) per *= 2;
         const dim3 g((unsigned)((rows + gr / per - 1) / (gr / per))), b(256);
-        if (D == 64) hipLaunchKernelGGL(quant_join_kernel<64>, g, b, 0, st, part_o, reinterpret_cast<const float2*>(part_ml), out, rows, p.slots, per);
-        else hipLaunchKernelGGL(quant_join_kernel<128>, g, b, 0, st, part_o, reinterpret_cast<const float2*>(part_ml), out, rows, p.slots, per);
+        if (D == 64) hipLaunchKernelGGL(quant_join_kernel<64>, g, b, 0, st, part_o, part_l, out, rows, p.slots, per);
+        else hipLaunchKernelGGL(quant_join_kernel<128>, g, b, 0, st, part_o, part_l, out, rows, p.slots, per);
     }
 }
 

@@ -72,6 +72,12 @@ MORE = [
     ("mxfp4", 128, 8, 1, 16, [333, 257, 90], [333, 128, 1]),
     ("int8", 64, 8, 8, 48, [300], [299]),
     ("mxfp4", 64, 32, 4, 16, [260, 40], [250, 40]),
+    ("int8", 128, 8, 1, 16, [2100], [40]),                      # tiles of 256 rows
+    ("mxfp4", 64, 16, 2, 32, [2050, 2100], [35, 33]),
+    ("int8", 64, 16, 1, 16, [2049], [20]),
+    ("int8", 128, 8, 2, 16, [1 + 97 * i % 1500 for i in range(20)] + [0, 1500], None),      # pieces of one size
+    ("mxfp4", 64, 8, 4, 16, [(31 * i * i) % 700 for i in range(150)], None),
+    ("mxfp4", 128, 16, 2, 64, [20] * 30 + [3000], None),
 ]
 
 
@@ -82,6 +88,39 @@ def test_attention(case):
     t.check_attention(out, q, cpu(cache), table, ctx.cpu(), None if q_start is None else q_start.cpu())
     assert not out[-3:].any()
     assert torch.equal(out, ops.quant_attention(q, cache, table, ctx, q_start))
+
+
+@pytest.mark.parametrize("lens", (None, [1, 90]), ids=("rows", "tiles"))
+@pytest.mark.parametrize("D", (64, 128))
+def test_scales_far_apart(D, lens):
+    """int8: value scales that grow and shrink by orders of magnitude along the keys, and scores that grow all the way, so that every step moves the maximum."""
+    q, cache, table, ctx, q_start = t.attention_case("int8", D, 8, 2, 16, [420, 400], lens, DEV)
+    at = torch.arange(cache.vs.numel(), device=DEV).view(cache.vs.shape)
+    cache.vs.mul_(torch.exp2(((at * 37) % 61 - 30).float()))
+    cache.vs[table[1, 3].long()] = 0                            # values of nothing
+    for b in range(2):
+        for i, p in enumerate(table[b, :-(-int(ctx[b]) // 16)].tolist()):
+            cache.ks[p] *= 1 + i
+    out = ops.quant_attention(q, cache, table, ctx, q_start)
+    want, size = plain.attention(q.cpu(), cpu(cache), table.cpu(), ctx.cpu(), None if q_start is None else q_start.cpu())
+    # Scores of up to 30 * 27: off by 2^-11 * 27 relative to the probabilities, and the roundings as ever.  Probabilities times scales are float16, a row's largest, W, at
+    # 2^7 or more: each is off by up to half of float16's least step, 2^-25 = 2^-32 W, times a code of up to 127; the largest's row has a code of 127, so 127 W is
+    # no more than the largest of the row's sizes.
+    least = 420 * 2 ** -32 * size.amax(-1, keepdim=True)
+    assert ((out.double().cpu() - want).abs() <= t.HALF * want.abs() + (t.HALF + 2 ** -6) * size + least + 1e-30).all()
+    cache.vs.fill_(0)
+    assert not ops.quant_attention(q, cache, table, ctx, q_start).any()
+
+
+@pytest.mark.parametrize("kind", t.KINDS)
+def test_tables_wider_than_contexts(kind):
+    """Work is cut up by the table, or by max_ctx; how codes are read (marked, from 192 MiB on) changes nothing."""
+    q, cache, table, ctx, _ = t.attention_case(kind, 128, 8, 2, 16, [500, 33], None, DEV)
+    want = ops.quant_attention(q, cache, table, ctx)
+    wide = torch.zeros(2, 40000, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    assert torch.equal(want, ops.quant_attention(q, cache, wide, ctx, max_ctx=table.shape[1] * 16))
+    t.check_attention(ops.quant_attention(q, cache, wide, ctx), q, cpu(cache), table, ctx.cpu(), None)
 
 
 # (kind, D, hq, hkv, page, whole shared pages of each group, sequences of each group, own tokens, tokens of each or None, sequences before and behind the groups)
