@@ -46,6 +46,7 @@ struct AttnArgs {
     float* part_l;            // [slots, T * hq]: base-2 logarithm of the sum of probabilities, -inf: no keys; part_o is what they average to
     int slots, splits, slot0;
     int page_shift;           // pages of a power of two tokens; -1: others
+    bool last;                // the sequences' own keys, after what their groups share, in one piece: joins both and writes the output
     int share;                // 0: every sequence's keys in `splits` pieces; else pieces of one size, about so many a key head (find_piece)
 };
 
@@ -445,7 +446,7 @@ __global__ void __launch_bounds__(256, NQT == 1 ? (KIND == kInt8 && D == 128 ? 3
     if (guess) pg.ask(a, a.bt + (int64_t)tile.item * a.bt_stride, w * 32, a.width * a.cache.page, lane);
     // the rows of this lane: the last position each sees, and its queries
     const Item<GROUPS> item(a, tile, lane);
-    if (split == 0) item.mark(a, tile, ROWS, h, G, 256);
+    if (split == 0 && !a.last) item.mark(a, tile, ROWS, h, G, 256);
     int rpos[NQT];
     bf16x8 qf[NQT][NC];
     int first = INT_MAX, last = -1;   // the last position that all rows of the tile see, and that any does
@@ -614,9 +615,32 @@ __global__ void __launch_bounds__(256, NQT == 1 ? (KIND == kInt8 && D == 128 ? 3
 #pragma unroll
     for (int qt = 0; qt < NQT; ++qt) {
         const float all = rows_sum(l[qt]), inv = all == 0.f ? 0.f : (KIND == kInt8 ? 1.f / kCodeUnit : 1.f) / all;
-        const float lse = all == 0.f ? -INFINITY : ref[qt] + __log2f(all);
+        float lse = all == 0.f ? -INFINITY : ref[qt] + __log2f(all);
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt) o[qt][dt] *= inv;
+        const int R = tile.at + 16 * qt + r;
+        const bool live = R < tile.toks * G;
+        const int64_t row = (int64_t)(tile.tok0 + R / G) * a.hq + h * G + R % G;
+        if constexpr (!GROUPS) {
+            if (a.last && item.k0 >= 0 && live) {   // the pieces of the group's keys, in turn over the waves; a wave's average of a piece and its own
+                for (int s = w; s < a.slot0; s += 4) {
+                    const int64_t at = (int64_t)s * a.T * a.hq + row;
+                    const float other = a.part_l[at];
+                    if (other == -INFINITY) continue;
+                    f32x4 x[4][ND / 4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int c = 0; c < ND / 4; ++c) x[i][c] = *reinterpret_cast<const f32x4*>(a.part_o + at * D + (4 * h4 + i) * ND + 4 * c);
+                    const float mx = fmaxf(lse, other), f = __builtin_amdgcn_exp2f(lse - mx), g = __builtin_amdgcn_exp2f(other - mx), both = 1.f / (f + g);
+                    lse = mx + __log2f(f + g);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int dt = 0; dt < ND; ++dt) o[qt][dt][i] = (o[qt][dt][i] * f + x[i][dt >> 2][dt & 3] * g) * both;
+                }
+            }
+        }
         const int owner = qt & 3;
         const int place = w < owner ? w : w - 1;
         if (qt) __syncthreads();
@@ -641,11 +665,8 @@ __global__ void __launch_bounds__(256, NQT == 1 ? (KIND == kInt8 && D == 128 ? 3
 #pragma unroll
                 for (int dt = 0; dt < ND; ++dt) o[qt][dt] += so[p][dt][lane] * f;
             }
-            const int R = tile.at + 16 * qt + r;
-            const bool live = R < tile.toks * G;
-            const int64_t row = (int64_t)(tile.tok0 + R / G) * a.hq + h * G + R % G;
             const float one = sum == 0.f ? 0.f : 1.f / sum;
-            if (live && a.slots == 1) {
+            if (live && (a.slots == 1 || a.last)) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint16_t* dst = a.out + row * D + (4 * h4 + i) * ND;
@@ -1111,17 +1132,20 @@ int tile_of(int64_t rows, int64_t items, int64_t keys) {
 AttnPlan quant_attention_plan(int T, int B, bool single, int groups, int hq, int heads, int64_t keys) {
     AttnPlan p{};
     const int64_t rows = (int64_t)T * (hq / heads);
-    auto side = [&](int64_t items, int& tile, int64_t& tiles, int& splits) {
+    auto side = [&](int64_t items, bool own, int& tile, int64_t& tiles, int& splits) {
         tile = tile_of(rows, items, keys);
         tiles = rows / tile + items + 1;
         const int64_t wgs = ((rows + tile - 1) / tile > items ? (rows + tile - 1) / tile : items) * heads;
-        const int64_t target = tile <= 32 ? 1024 : 256, least = tile <= 32 ? 256 : tile / 2;
-        int64_t s = tile <= 32 ? (target + wgs - 1) / wgs : (target + wgs / 2) / wgs;
+        // by rows of 16 and 32: two workgroups a CU are enough without pieces, whose sums take a launch to join (64 rows of 2048 keys and 8 heads: 49 us, with two pieces each
+        // 57); pieces of fewer keys than `least` gain nothing.  By tiles: a workgroup a CU, with two the sums' way through memory costs more (64 rows on 8192 shared keys: 43 us
+        // against 37).  What sequences have of their own behind a shared prefix is taken to be short.
+        const int64_t least = tile > 32 ? tile / 2 : own && groups > 0 ? 2048 : 256;
+        int64_t s = tile <= 32 ? (wgs >= 512 ? 1 : (1024 + wgs - 1) / wgs) : (256 + wgs / 2) / wgs;
         s = s < (keys + least - 1) / least ? s : (keys + least - 1) / least;
         splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
     };
-    side(B, p.own_rows, p.own_tiles, p.own_splits);
-    if (groups > 0) side(groups, p.group_rows, p.group_tiles, p.group_splits);
+    side(B, true, p.own_rows, p.own_tiles, p.own_splits);
+    if (groups > 0) side(groups, false, p.group_rows, p.group_tiles, p.group_splits);
     p.slots = p.own_splits + p.group_splits;
     // few sequences of one token each, whose lengths decide how long the card is busy: pieces of one size
     if (single && groups == 0 && B >= 16 && B <= 256 && p.own_rows >= hq / heads && p.own_splits > 1) {
@@ -1138,7 +1162,7 @@ void launch_quant_attention(int kind, int D, const AttnPlan& p, const uint16_t* 
     if (T == 0) return;
     AttnArgs a{q, q_stride, cache, bt, bt_stride, width, q_start, ctx_len, groups ? group_start : nullptr, prefix_len, B, T, groups, hq, scale * 1.4426950408889634f,
                out, part_o, part_l, p.slots, 0, 0,
-               (cache.page & (cache.page - 1)) ? -1 : __builtin_ctz(cache.page), 0};
+               (cache.page & (cache.page - 1)) ? -1 : __builtin_ctz(cache.page), false, 0};
     if (groups) {
         a.splits = p.group_splits;
         a.slot0 = 0;
@@ -1148,9 +1172,10 @@ void launch_quant_attention(int kind, int D, const AttnPlan& p, const uint16_t* 
     a.share = p.share;
     a.slot0 = p.group_splits;
     // one token of each sequence: tiles are counted without a look at where sequences begin
+    a.last = groups && p.own_rows <= 32 && p.own_splits == 1;
     const int64_t tiles = q_start || p.share ? p.own_tiles : (int64_t)T * ((hq / cache.heads + p.own_rows - 1) / p.own_rows);
     launch_rows_of<false>(kind, D, p.own_rows, a, tiles, st);
-    if (p.slots > 1) {
+    if (p.slots > 1 && !a.last) {
         const int64_t rows = (int64_t)T * hq;
         const int gr = 256 / (D / 4);
         int per = 1;   // lanes' groups of a row: the rows fill the card with one, or there are pieces to share
