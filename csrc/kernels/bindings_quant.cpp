@@ -6,6 +6,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <tuple>
 
 #include "chronos_quant_kv.h"
@@ -151,12 +152,13 @@ Tensor quant_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
     const int64_t keys = block_table.size(1) * c.c.page;
     CHK(keys < kMost, "block_table is too wide");
     c10::hip::HIPGuardMasqueradingAsCUDA g(k.device());
+    if (T == 0 || B == 0 || keys == 0) return at::zeros({T, hq, D}, q.options());
+    const auto p = chronos::qkv::quant_attention_plan((int)T, (int)B, qs == nullptr, (int)groups, (int)hq, (int)heads, max_ctx > 0 && max_ctx < keys ? max_ctx : keys);
+    // a launch has fewer than 2^32 threads: up to 512 a tile and head, and 32 a row of the one that joins
+    CHK(std::max(p.own_tiles, p.group_tiles) * heads < (1 << 23) && T * hq < (1 << 27), "too many tokens or sequences for one call");
     auto out = at::empty({T, hq, D}, q.options());
-    if (T == 0) return out;
-    if (B == 0 || keys == 0) return out.zero_();
     const bool rows = q.stride(2) == 1 && q.stride(1) == D && q.stride(0) % 8 == 0 && q.stride(0) >= 0 && (uintptr_t)q.data_ptr() % 16 == 0;
     const Tensor x = rows ? q : q.clone(at::MemoryFormat::Contiguous);
-    const auto p = chronos::qkv::quant_attention_plan((int)T, (int)B, qs == nullptr, (int)groups, (int)hq, (int)heads, max_ctx > 0 && max_ctx < keys ? max_ctx : keys);
     Tensor po, pm;
     if (p.slots > 1) {
         po = at::empty({p.slots, T * hq, D}, q.options().dtype(at::kFloat));

@@ -152,7 +152,7 @@ template <bool GROUPS> struct Item {
         } else {
             s0 = t;
         }
-        return min(a.ctx_len[s0], a.width * a.cache.page) - first_row(a, s0 + 1) + t;
+        return min(max(a.ctx_len[s0], 0), a.width * a.cache.page) - first_row(a, s0 + 1) + t;
     }
     // keys [k0, the end) of rows that see up to `last`; a piece of them
     __device__ __forceinline__ void piece(const AttnArgs& a, const Tile& tile, int last, int split, int unit, int& from, int& to) const {
@@ -1145,6 +1145,8 @@ AttnPlan quant_attention_plan(int T, int B, bool single, int groups, int hq, int
         splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
     };
     side(B, true, p.own_rows, p.own_tiles, p.own_splits);
+    // one token of each sequence: tiles are counted without a look at where sequences begin
+    if (single) p.own_tiles = (int64_t)T * ((hq / heads + p.own_rows - 1) / p.own_rows);
     if (groups > 0) side(groups, false, p.group_rows, p.group_tiles, p.group_splits);
     p.slots = p.own_splits + p.group_splits;
     // few sequences of one token each, whose lengths decide how long the card is busy: pieces of one size
@@ -1171,10 +1173,8 @@ void launch_quant_attention(int kind, int D, const AttnPlan& p, const uint16_t* 
     a.splits = p.share ? 1 : p.own_splits;
     a.share = p.share;
     a.slot0 = p.group_splits;
-    // one token of each sequence: tiles are counted without a look at where sequences begin
     a.last = groups && p.own_rows <= 32 && p.own_splits == 1;
-    const int64_t tiles = q_start || p.share ? p.own_tiles : (int64_t)T * ((hq / cache.heads + p.own_rows - 1) / p.own_rows);
-    launch_rows_of<false>(kind, D, p.own_rows, a, tiles, st);
+    launch_rows_of<false>(kind, D, p.own_rows, a, p.own_tiles, st);
     if (p.slots > 1 && !a.last) {
         const int64_t rows = (int64_t)T * hq;
         const int gr = 256 / (D / 4);

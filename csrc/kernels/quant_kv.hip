@@ -263,13 +263,18 @@ void launch_norm_rope_kv_quant(int kind, int D, const uint16_t* qkv, int64_t qkv
     // four head rows a lane where the card is full all the same
     const bool four = T * ((hq + 4 * side - 1) / (4 * side)) >= 1024;
     const int q_parts = (hq + (four ? 4 : 1) * side - 1) / ((four ? 4 : 1) * side), parts = q_parts + (2 * cache.heads + side - 1) / side;
-    const dim3 g((unsigned)(T * parts)), b(256);
+    const dim3 b(256);
+    // a launch has fewer than 2^32 threads
+    const int64_t most = (1 << 23) / parts > 0 ? (1 << 23) / parts : 1;
+    for (int64_t t = 0; t < T; t += most) {
+        const dim3 g((unsigned)((T - t < most ? T - t : most) * parts));
 #define CHRONOS_QKV(K, DD, N)                                                                                                                                        \
     if (kind == K && D == DD && four == (N == 4))                                                                                                                    \
-        hipLaunchKernelGGL((norm_rope_kv_quant_kernel<K, DD, N>), g, b, 0, st, qkv, qkv_stride, pos, tok_seq, bt, bt_stride, seqs, width, cos_sin, R, P, q_norm,     \
-                           k_norm, eps, q_out, cache, hq, q_parts, parts);
-    CHRONOS_QKV(kInt8, 64, 1) CHRONOS_QKV(kInt8, 128, 1) CHRONOS_QKV(kFp4, 64, 1) CHRONOS_QKV(kFp4, 128, 1)
-    CHRONOS_QKV(kInt8, 64, 4) CHRONOS_QKV(kInt8, 128, 4) CHRONOS_QKV(kFp4, 64, 4) CHRONOS_QKV(kFp4, 128, 4)
+        hipLaunchKernelGGL((norm_rope_kv_quant_kernel<K, DD, N>), g, b, 0, st, qkv + t * qkv_stride, qkv_stride, pos + t, tok_seq + t, bt, bt_stride, seqs, width,   \
+                           cos_sin, R, P, q_norm, k_norm, eps, q_out + t * hq * D, cache, hq, q_parts, parts);
+        CHRONOS_QKV(kInt8, 64, 1) CHRONOS_QKV(kInt8, 128, 1) CHRONOS_QKV(kFp4, 64, 1) CHRONOS_QKV(kFp4, 128, 1)
+        CHRONOS_QKV(kInt8, 64, 4) CHRONOS_QKV(kInt8, 128, 4) CHRONOS_QKV(kFp4, 64, 4) CHRONOS_QKV(kFp4, 128, 4)
+    }
 #undef CHRONOS_QKV
 }
 

@@ -9,8 +9,8 @@ Beside the bf16 / e4m3 pages of ``rope_kv_write`` and ``paged_attention``, whose
 Heads have 64 or 128 dimensions, pages a multiple of 16 tokens, query heads are any multiple of the cache's.  Every function takes GPU tensors (the HIP kernels of
 csrc/kernels/quant_kv.hip and quant_attention.hip; current stream, captured into graphs as other launches are) or CPU tensors (:mod:`.quant_kv_ref`).
 
-What is not there is left out: a token whose position is negative, or whose page the table or the cache does not have, is not written and reads as zeros (so padded
-batches need no page of their own); keys on pages outside the cache (say -1) are not seen; a query row that sees no key is zeros.  A head row with an infinity or NaN is
+What is not there is left out: a token whose position is negative or (as it is written) behind the rope table, or whose page the table or the cache does not have, is not
+written and reads as zeros (so padded batches need no page of their own); keys on pages outside the cache (say -1) are not seen; a query row that sees no key is zeros.  A head row with an infinity or NaN is
 held as NaN as a whole, and makes NaN of the rows that see it, of no others.
 """
 from __future__ import annotations

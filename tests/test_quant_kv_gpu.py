@@ -297,3 +297,36 @@ def test_offsets_past_32_bits(kind, D):
         assert torch.equal(a, b)
     for a, b in zip((cache.k, cache.v, cache.ks, cache.vs), (small.k, small.v, small.ks, small.vs)):
         assert torch.equal(a[-40:], b)
+
+
+def test_more_tokens_than_a_launch_has():
+    """2^24 tokens and some, most of them padding; and for the attention, which takes fewer, a refusal before anything is made."""
+    n, D = (1 << 24) + 3, 64
+    cache = ops.quant_kv_cache(2, 16, 1, D, "int8", DEV)
+    qkv = torch.zeros(n, 2 * D, dtype=torch.bfloat16, device=DEV)
+    pos, seq = torch.full((n,), -1, dtype=torch.int32, device=DEV), torch.zeros(n, dtype=torch.int32, device=DEV)
+    table, cs = t.ints([[1, 0]]).to(DEV), t.rope(32, D).to(DEV)
+    live = [0, 1 << 23, (1 << 23) + 1, n - 1]
+    x = t.rows_of(4, 2, D).flatten(1).to(DEV)
+    pos[live], qkv[live] = t.ints([3, 17, 4, 30]).to(DEV), x
+    assert ops.norm_rope_kv_quant(qkv, pos, seq, table, cs, cache, 0).shape == (n, 0, D)
+    small = ops.quant_kv_cache(2, 16, 1, D, "int8", DEV)
+    ops.norm_rope_kv_quant(x, pos[live], seq[:4], table, cs, small, 0)
+    assert all(torch.equal(a, b) for a, b in zip((cache.k, cache.v, cache.ks, cache.vs), (small.k, small.v, small.ks, small.vs))) and cache.k.any()
+    q = torch.zeros(1, 1, D, dtype=torch.bfloat16, device=DEV).expand(n, 1, D)
+    with pytest.raises(RuntimeError, match="too many tokens or sequences"):
+        ops.quant_attention(q, cache, table.expand(n, 2), seq)
+    with pytest.raises(RuntimeError, match="too many tokens or sequences"):
+        ops.quant_attention(q.expand(n, 16, D), cache, table, seq[:1], t.ints([0, n]).to(DEV))
+
+
+def test_contexts_of_less_than_nothing():
+    """The least number that a length can be, in a group and outside: rows that see nothing."""
+    (q, table, ctx, groups, prefix, q_start), cache = prefix_case("int8", 128, 8, 2, 16, [6], [4], [9, 2, 3, 40], [3, 2, 1, 3], 1)
+    want = ops.prefix_attention(q, cache, table, ctx, groups, prefix, q_start)
+    ctx[0] = ctx[2] = -(1 << 31)
+    got = ops.prefix_attention(q, cache, table, ctx, groups, prefix, q_start)
+    rows = q_start.tolist()
+    for b in range(6):
+        a, e = rows[b], rows[b + 1]
+        assert not got[a:e].any() if b in (0, 2) else torch.equal(got[a:e], want[a:e])
