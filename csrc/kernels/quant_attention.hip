@@ -47,6 +47,7 @@ struct AttnArgs {
     int slots, splits, slot0;
     int page_shift;           // pages of a power of two tokens; -1: others
     bool last;                // the sequences' own keys, after what their groups share, in one piece: joins both and writes the output
+    bool longest;             // tiles by the number of their keys, most first (find_longest)
     int share;                // 0: every sequence's keys in `splits` pieces; else pieces of one size, about so many a key head (find_piece)
 };
 
@@ -103,6 +104,67 @@ template <bool GROUPS> __device__ __forceinline__ bool find_tile(const AttnArgs&
             out.tok0 = __builtin_amdgcn_readlane(t0, l);
             out.toks = __builtin_amdgcn_readlane(t1, l) - out.tok0;
             out.at = (index - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(tiles, l))) * rows;
+            return true;
+        }
+        before += total;
+    }
+    return false;
+}
+// Tile `index` of up to 255 sequences' tiles, those with most keys first (within 32): where tiles are more than the card holds at a time, a prompt's last ones, which are
+// its longest, are not what all others wait for.  Every wave finds it by itself, halving the range of lengths: count() tiles have more than 32 `level` keys.
+__device__ __forceinline__ bool find_longest(const AttnArgs& a, int index, int G, int rows, int lane, Tile& out) {
+    constexpr int CH = 4;
+    int t0[CH], n[CH], ctx[CH], most = 0;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int seq = i * 64 + lane;
+        t0[i] = seq <= a.B ? first_row(a, seq) : a.T;
+        n[i] = seq <= a.B ? max(first_row(a, seq + 1) - t0[i], 0) : 0;
+        ctx[i] = seq < a.B ? (int)min((int64_t)max(a.ctx_len[seq], 0), (int64_t)a.width * a.cache.page) : 0;
+        most = max(most, ctx[i]);
+    }
+    const int shift = __builtin_ctz(rows);   // a power of two
+    auto of = [&](int i, int level) {   // tiles of item i * 64 + lane with more than 32 level keys: its last ones
+        const int tiles = (n[i] * G + rows - 1) >> shift, more = level * 32 - ctx[i] + n[i];
+        return level < 0 ? tiles : ctx[i] <= level * 32 ? 0 : tiles - min(more > 0 ? (more * G) >> shift : 0, max(tiles - 1, 0));
+    };
+    auto count = [&](int level) {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+            if (i * 64 <= a.B) c += of(i, level);
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) c += __shfl_xor(c, o, 64);
+        return __builtin_amdgcn_readfirstlane(c);
+    };
+    if (index >= count(-1)) return false;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o, 64));
+    int low = -1, high = __builtin_amdgcn_readfirstlane(most) / 32 + 1;   // count(low) > index >= count(high)
+    while (high - low > 1) {
+        const int mid = (low + high) >> 1;
+        if (count(mid) > index) low = mid;
+        else high = mid;
+    }
+    int before = count(high);   // the tile is one of those with more than 32 low keys and no more than 32 high
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        if (i * 64 > a.B) break;
+        const int some = of(i, low), here = some - of(i, high);
+        int upto = here;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(upto, o, 64);
+            if (lane >= o) upto += v;
+        }
+        const int total = __builtin_amdgcn_readlane(upto, 63);
+        if (index < before + total) {
+            const int l = __builtin_ctzll(__ballot(before + upto > index));
+            out.item = i * 64 + l;
+            out.tok0 = __builtin_amdgcn_readlane(t0[i], l);
+            out.toks = __builtin_amdgcn_readlane(n[i], l);
+            const int tiles = (out.toks * G + rows - 1) >> shift;
+            out.at = (tiles - __builtin_amdgcn_readlane(some, l) + index - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(here, l))) << shift;
             return true;
         }
         before += total;
@@ -714,15 +776,15 @@ template <int KIND, int D> struct Fetch {
     uint32_t w[8 * VW > 4 * NP ? 8 * VW : 4 * NP];   // keys: 4 words of each piece; values: VW of each key
     uint32_t e[KIND == kFp4 ? 8 : 1];                // mxfp4: E of the pieces' blocks, or the words of the eight keys' values
     uint32_t scale;                                  // keys' waves, int8: lane i < 32: of key i, i >= 32: its value's; mxfp4: the word of key i's value
-    int blk[2], t0;
+    int blk0, blk1, t0;                              // pages of the first 16 keys and of the others, -1: not there; the first key
 
-    __device__ __forceinline__ int64_t row_of(const AttnArgs& a, int g, int h) const {
-        return ((int64_t)max(blk[g], 0) * a.cache.heads + h) * a.cache.page + Pages::off(a, t0 + 16 * g);
+    static __device__ __forceinline__ int64_t row_of(const AttnArgs& a, int blk, int at, int h) {
+        return ((int64_t)max(blk, 0) * a.cache.heads + h) * a.cache.page + Pages::off(a, at);
     }
     __device__ __forceinline__ void keys(const AttnArgs& a, const Pages& pg, int at, int h, int lane) {
         t0 = at;
-        blk[0] = pg.blk(a, 0), blk[1] = pg.blk(a, 1);
-        const int64_t row0 = row_of(a, 0, h), row1 = row_of(a, 1, h);
+        blk0 = pg.blk(a, 0), blk1 = pg.blk(a, 1);
+        const int64_t row0 = row_of(a, blk0, at, h), row1 = row_of(a, blk1, at + 16, h);
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
             constexpr int KP = 1024 / RB;   // keys of a piece
@@ -740,9 +802,9 @@ template <int KIND, int D> struct Fetch {
     }
     __device__ __forceinline__ void values(const AttnArgs& a, const Pages& pg, int at, int h, int lane) {
         t0 = at;
-        blk[0] = pg.blk(a, 0), blk[1] = pg.blk(a, 1);
+        blk0 = pg.blk(a, 0), blk1 = pg.blk(a, 1);
         const int r = lane & 15, h2 = lane >> 4 & 1;
-        const int64_t row = (lane < 32 ? row_of(a, 0, h) : row_of(a, 1, h)) + 4 * h2;
+        const int64_t row = (lane < 32 ? row_of(a, blk0, at, h) : row_of(a, blk1, at + 16, h)) + 4 * h2;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const uint8_t* vp = a.cache.v + (row + (j & 3) + 8 * (j >> 2)) * RB + (RB / 16) * r;
@@ -772,7 +834,7 @@ template <int KIND, int D> struct Fetch {
     // keys 32 i .. of the step
     template <int WAVES> __device__ __forceinline__ void put_keys(TileStep<KIND, D, WAVES>& s, int i, int end, float scale_log2, int lane) const {
         const uint32_t in = t0 >= end ? 0u : end - t0 >= 32 ? ~0u : (1u << (end - t0)) - 1u;
-        const uint32_t there = in & ((blk[0] >= 0 ? 0xffffu : 0u) | (blk[1] >= 0 ? 0xffff0000u : 0u));
+        const uint32_t there = in & ((blk0 >= 0 ? 0xffffu : 0u) | (blk1 >= 0 ? 0xffff0000u : 0u));
         const int key = lane & 31;
         const bool here = there >> key & 1;
         if constexpr (KIND == kInt8) {
@@ -842,7 +904,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
     const int heads = a.cache.heads, G = a.hq / heads;
     const int h = blockIdx.x % heads, split = blockIdx.y;
     Tile tile;
-    if (!find_tile<GROUPS>(a, blockIdx.x / heads, G, ROWS, lane, tile)) return;
+    if (!GROUPS && a.longest) {
+        if (!find_longest(a, blockIdx.x / heads, G, ROWS, lane, tile)) return;
+    } else if (!find_tile<GROUPS>(a, blockIdx.x / heads, G, ROWS, lane, tile)) {
+        return;
+    }
     tile.same();
     const Item<GROUPS> item(a, tile, lane);
     if (split == 0) item.mark(a, tile, ROWS, h, G, 64 * WAVES);
@@ -1164,7 +1230,7 @@ void launch_quant_attention(int kind, int D, const AttnPlan& p, const uint16_t* 
     if (T == 0) return;
     AttnArgs a{q, q_stride, cache, bt, bt_stride, width, q_start, ctx_len, groups ? group_start : nullptr, prefix_len, B, T, groups, hq, scale * 1.4426950408889634f,
                out, part_o, part_l, p.slots, 0, 0,
-               (cache.page & (cache.page - 1)) ? -1 : __builtin_ctz(cache.page), false, 0};
+               (cache.page & (cache.page - 1)) ? -1 : __builtin_ctz(cache.page), false, false, 0};
     if (groups) {
         a.splits = p.group_splits;
         a.slot0 = 0;
@@ -1174,6 +1240,8 @@ void launch_quant_attention(int kind, int D, const AttnPlan& p, const uint16_t* 
     a.share = p.share;
     a.slot0 = p.group_splits;
     a.last = groups && p.own_rows <= 32 && p.own_splits == 1;
+    // tiles of 256 rows have a CU each, of 128 half of one
+    a.longest = q_start && !groups && B < 256 && p.own_rows > 32 && p.own_tiles * cache.heads > (p.own_rows == 256 ? 256 : 512);
     launch_rows_of<false>(kind, D, p.own_rows, a, p.own_tiles, st);
     if (p.slots > 1 && !a.last) {
         const int64_t rows = (int64_t)T * hq;

@@ -90,6 +90,25 @@ def test_attention(case):
     assert torch.equal(out, ops.quant_attention(q, cache, table, ctx, q_start))
 
 
+# more tiles than the card holds at a time, which go by their lengths: (kind, D, hq, hkv, page, contexts, tokens, keys that the table has room for)
+LONGEST = [
+    ("int8", 64, 64, 64, 16, [300, 0, 517, 129, 64, 700], [300, 0, 260, 129, 5, 600], 0),
+    ("mxfp4", 64, 128, 32, 32, [400, 90, 33], [333, 90, 133], 2080),       # tiles of 256 rows
+    ("mxfp4", 128, 64, 64, 16, [7, 250] + [(37 * i) % 200 for i in range(70)], [9, 40] + [(37 * i) % 200 // 3 + 5 for i in range(70)], 0),   # more tokens than context, too
+    ("int8", 128, 96, 32, 16, [(53 * i) % 97 for i in range(254)] + [300], [11] * 255, 0),      # as many sequences as there may be
+]
+
+
+@pytest.mark.parametrize("case", LONGEST, ids=lambda c: "-".join(map(str, c[:5])) + f"-{len(c[5])}")
+def test_longest_first(case):
+    q, cache, table, ctx, q_start = t.attention_case(*case[:7], DEV, tail=3)
+    wide = torch.zeros(table.shape[0], max(table.shape[1], case[7] // case[4]), dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    out = ops.quant_attention(q, cache, wide, ctx, q_start)
+    t.check_attention(out, q, cpu(cache), table, ctx.cpu(), q_start.cpu())
+    assert not out[-3:].any()
+
+
 @pytest.mark.parametrize("lens", (None, [1, 90]), ids=("rows", "tiles"))
 @pytest.mark.parametrize("D", (64, 128))
 def test_scales_far_apart(D, lens):
