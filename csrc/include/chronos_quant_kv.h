@@ -23,9 +23,9 @@ struct Cache {
 };
 
 // How a call of the attention is cut up (quant_attention.hip): rows of a tile, tiles and pieces of the keys, for the sequences' own keys and for those that
-// groups share; slots of partial sums, 1: none; share: pieces of one size, about so many a key head
+// groups share; slots of partial sums, 1: none
 struct AttnPlan {
-    int own_rows, own_splits, group_rows, group_splits, slots, share;
+    int own_rows, own_splits, group_rows, group_splits, slots;
     int64_t own_tiles, group_tiles;
 };
 

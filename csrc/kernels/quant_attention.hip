@@ -48,7 +48,6 @@ struct AttnArgs {
     int page_shift;           // pages of a power of two tokens; -1: others
     bool last;                // the sequences' own keys, after what their groups share, in one piece: joins both and writes the output
     bool longest;             // tiles by the number of their keys, most first (find_longest)
-    int share;                // 0: every sequence's keys in `splits` pieces; else pieces of one size, about so many a key head (find_piece)
 };
 
 namespace {
@@ -238,70 +237,6 @@ template <bool GROUPS> struct Item {
     }
 };
 
-// One token of each of up to 256 sequences, of lengths that may be far apart: their keys in pieces of one size, a multiple of 128 keys, for about a.share workgroups a
-// key head, at most `slots` a sequence.  Piece `index` of the sequences' pieces in order; behind them the tokens of no sequence.  Every wave counts by itself.
-struct Piece {
-    int seq, split, splits, keys;   // seq: or the token, from B on; keys: of a piece
-};
-__device__ __forceinline__ int lanes_scan(int v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(v, o, 64);
-        if (lane >= o) v += u;
-    }
-    return v;
-}
-__device__ __forceinline__ bool find_piece(const AttnArgs& a, int index, int lane, Piece& out) {
-    constexpr int CH = 4;
-    int units[CH], sum = 0, most = 0;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-        const int seq = i * 64 + lane;
-        units[i] = seq < a.B ? (int)((min((int64_t)max(a.ctx_len[seq], 0), (int64_t)a.width * a.cache.page) + 127) >> 7) : 0;
-        sum += units[i];
-        most = max(most, units[i]);
-    }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        sum += __shfl_xor(sum, o, 64);
-        most = max(most, __shfl_xor(most, o, 64));
-    }
-    sum = __builtin_amdgcn_readfirstlane(sum);
-    most = __builtin_amdgcn_readfirstlane(most);
-    const int size = max(max((sum + a.share - 1) / a.share, (most + a.slots - 1) / a.slots), 1);
-    const float inv = 1.f / (float)size;
-    int full[CH], all = 0;   // whole pieces; they come first, the sequences' rests (also of none) when places become free
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-        int n = (int)((float)units[i] * inv);   // units up to 2^23: a quotient that is off by one is put right
-        n += (n + 1) * size <= units[i];
-        full[i] = n - (n * size > units[i]);
-        all += full[i];
-    }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) all += __shfl_xor(all, o, 64);
-    all = __builtin_amdgcn_readfirstlane(all);
-    const bool rests = index >= all;
-    int before = rests ? all : 0;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-        if (i * 64 >= a.B) break;
-        const int rest = i * 64 + lane < a.B && (full[i] * size < units[i] || units[i] == 0), n = rests ? rest : full[i];
-        const int upto = lanes_scan(n, lane), total = __builtin_amdgcn_readlane(upto, 63);
-        if (index < before + total) {
-            const int l = __builtin_ctzll(__ballot(before + upto > index)), f = __builtin_amdgcn_readlane(full[i], l);
-            out.seq = i * 64 + l;
-            out.splits = f + __builtin_amdgcn_readlane(rest, l);
-            out.split = rests ? f : index - before - (__builtin_amdgcn_readlane(upto, l) - f);
-            out.keys = size * 128;
-            return true;
-        }
-        before += total;
-    }
-    out = Piece{a.B + index - before, 0, 1, 128};
-    return out.seq < a.T;
-}
-
 // ---- codes to operands --------------------------------------------------------------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -486,25 +421,13 @@ __global__ void __launch_bounds__(256, NQT == 1 ? (KIND == kInt8 && D == 128 ? 3
     const int r = lane & 15, h4 = lane >> 4;
     const int heads = a.cache.heads, G = a.hq / heads;
     const int h = blockIdx.x % heads;
-    int split = blockIdx.y;
+    const int split = blockIdx.y;
     Tile tile;
-    Piece own{0, 0, 0, 0};
-    if (!GROUPS && a.share) {
-        if (!find_piece(a, blockIdx.x / heads, lane, own)) return;
-        tile = Tile{min(own.seq, a.B), own.seq, 1, 0};
-        split = own.split;
-        if (split == 0)   // the slots that its rows have no pieces for
-            for (int i = threadIdx.x; i < G * (a.slots - own.splits); i += 256)
-                a.part_l[(int64_t)(own.splits + i / G) * a.T * a.hq + (int64_t)own.seq * a.hq + h * G + i % G] = -INFINITY;
-    } else if (!find_tile<GROUPS>(a, blockIdx.x / heads, G, ROWS, lane, tile)) {
-        return;
-    }
-
+    if (!find_tile<GROUPS>(a, blockIdx.x / heads, G, ROWS, lane, tile)) return;
     tile.same();
-    split = __builtin_amdgcn_readfirstlane(split);
     // keys from the first on, if no piece is cut: the wave's first pages do not wait for the context's length
     Pages pg{-1};
-    const bool guess = !GROUPS && !a.share && a.splits == 1 && !a.group_start && tile.item < a.B;
+    const bool guess = !GROUPS && a.splits == 1 && !a.group_start && tile.item < a.B;
     if (guess) pg.ask(a, a.bt + (int64_t)tile.item * a.bt_stride, w * 32, a.width * a.cache.page, lane);
     // the rows of this lane: the last position each sees, and its queries
     const Item<GROUPS> item(a, tile, lane);
@@ -543,12 +466,7 @@ __global__ void __launch_bounds__(256, NQT == 1 ? (KIND == kInt8 && D == 128 ? 3
         last = __builtin_amdgcn_readfirstlane(item.ctx - tile.toks + min(tile.toks - 1, (tile.at + ROWS - 1) / G));
     }
     int ks, ke;
-    if (!GROUPS && a.share) {
-        ks = split * own.keys;
-        ke = min(last + 1, ks + own.keys);
-    } else {
-        item.piece(a, tile, last, split, 128, ks, ke);
-    }
+    item.piece(a, tile, last, split, 128, ks, ke);
     const int32_t* bt = a.bt + (int64_t)item.seq * a.bt_stride;
     float ref[NQT], l[NQT];   // sums are of 2^(score - ref)
     f32x4 o[NQT][ND];
@@ -1170,9 +1088,11 @@ template <int KIND, int D, bool GROUPS> void launch_rows(int rows, const AttnArg
     } else if (rows == 32) {
         hipLaunchKernelGGL((quant_rows_kernel<KIND, D, 2, GROUPS, false>), g, b, 0, st, a);
     } else if (rows == 128) {
-        constexpr int lds = 2 * sizeof(TileStep<KIND, D, 4>);
-        lds_limit<quant_tile_kernel<KIND, D, 4, GROUPS>>(lds);
-        hipLaunchKernelGGL((quant_tile_kernel<KIND, D, 4, GROUPS>), g, b, lds, st, a);
+        if constexpr (GROUPS) {
+            constexpr int lds = 2 * sizeof(TileStep<KIND, D, 4>);
+            lds_limit<quant_tile_kernel<KIND, D, 4, true>>(lds);
+            hipLaunchKernelGGL((quant_tile_kernel<KIND, D, 4, true>), g, b, lds, st, a);
+        }
     } else {
         constexpr int lds = 2 * sizeof(TileStep<KIND, D, 8>);
         lds_limit<quant_tile_kernel<KIND, D, 8, GROUPS>>(lds);
@@ -1186,10 +1106,22 @@ template <bool GROUPS> void launch_rows_of(int kind, int D, int rows, const Attn
     else launch_rows<kFp4, 128, GROUPS>(rows, a, tiles, st);
 }
 
-// Rows of a tile, by the rows that an item has on average, and the keys
-int tile_of(int64_t rows, int64_t items, int64_t keys) {
+// workgroups of a launch with tiles of `tile` rows, without pieces, if the items' rows are alike
+int64_t groups_of(int64_t rows, int64_t items, int heads, int tile) {
+    const int64_t tiles = (rows + tile - 1) / tile;
+    return (tiles > items ? tiles : items) * heads;
+}
+// Rows of a tile, by the rows that an item has on average and the workgroups that this makes.  Small tiles read the keys more often, and large ones leave CUs idle and rows
+// empty.  Sequences (32 query and 8 key heads of 128, int8; 16 / 32 / 128 / 256 rows): 8 x 64 rows on 2000 keys 25 / 31 / 69 / 56 us; 32 x 64 on 2000 65 / 46 / 94 / 76;
+// 32 x 128 on 2000 112 / 82 / 96 / 77; 4 x 512 on 500 24 / 18 / 27 / 28.  What a group shares (4 rows a sequence and key head): 16 sequences on 2048 keys 20 / 21 / 26 / 27,
+// 64 on 8192 48 / 38 / 50 / 45, 128 on 16384 - / 107 / 92 / 112, two groups of those - / - / 149 / 130.
+int tile_of(int64_t rows, int64_t items, int heads, int64_t keys, bool own) {
     const int64_t per = items > 0 ? rows / items : rows;
-    return per <= 16 ? 16 : per <= 32 ? 32 : per <= 128 || keys < 2048 ? 128 : 256;
+    if (per <= 16) return 16;
+    // 1 x 128 rows on 16000 keys: 43 us in 16 pieces with 16 rows, 34 with 32; 2 x 64 sequences of 8 rows on 8192, one key head: 37 and 30
+    if (groups_of(rows, items, heads, 16) <= (own ? 256 : 64) && (own ? per <= 64 || keys < 4096 : per <= 128)) return 16;
+    if (per >= 112 && groups_of(rows, items, heads, 256) >= (own ? 128 : 32)) return 256;
+    return !own && per >= 192 && groups_of(rows, items, heads, 256) >= 16 ? 128 : 32;
 }
 
 }  // namespace
@@ -1199,14 +1131,27 @@ AttnPlan quant_attention_plan(int T, int B, bool single, int groups, int hq, int
     AttnPlan p{};
     const int64_t rows = (int64_t)T * (hq / heads);
     auto side = [&](int64_t items, bool own, int& tile, int64_t& tiles, int& splits) {
-        tile = tile_of(rows, items, keys);
+        tile = tile_of(rows, items, heads, keys, own);
         tiles = rows / tile + items + 1;
-        const int64_t wgs = ((rows + tile - 1) / tile > items ? (rows + tile - 1) / tile : items) * heads;
-        // by rows of 16 and 32: two workgroups a CU are enough without pieces, whose sums take a launch to join (64 rows of 2048 keys and 8 heads: 49 us, with two pieces each
-        // 57); pieces of fewer keys than `least` gain nothing.  By tiles: a workgroup a CU, with two the sums' way through memory costs more (64 rows on 8192 shared keys: 43 us
-        // against 37).  What sequences have of their own behind a shared prefix is taken to be short.
-        const int64_t least = tile > 32 ? tile / 2 : own && groups > 0 ? 2048 : 256;
-        int64_t s = tile <= 32 ? (wgs >= 512 ? 1 : (1024 + wgs - 1) / wgs) : (256 + wgs / 2) / wgs;
+        const int64_t wgs = groups_of(rows, items, heads, tile), full = tile == 256 ? 256 : 512;   // a workgroup a CU, or two
+        int64_t s = full / wgs, least = 256;
+        if (own) {
+            const int64_t busy = rows > 16 * items ? 160 : 224;
+            // Pieces take a launch to join.  Without any, a wave has 1000 keys in 8 us (2 x 700 keys: 9 us, with pieces 11; 16 x 1024: 10 and 12).  From `busy` workgroups on the
+            // card is busy enough (8 key heads, int8: 32 sequences of 2048 25 us, in two pieces 28, four 29; 24 of 500 to 2048 in four 20, in one 23), but for contexts that may be
+            // long, of which one may be far longer than the others (32 of 2048 to 8192 in four pieces 81, in two 82; of 8192 each 98 and 95;
+            // 8 x 96 rows on 2000 in tiles of 32 31 in one piece, 37 in four).
+            if (tile == 256) s = (full + wgs / 2) / wgs;
+            else if (wgs > 96) s = wgs < busy ? 768 / wgs : keys >= 4096 ? 1024 / wgs : 1;
+            const int64_t longest = wgs < full ? 4096 : 16 * wgs;   // of a piece; the more there is beside it the longer one may take
+            if (tile < 256 && keys / longest > s) s = keys / longest;
+            if (keys <= (wgs > 96 ? 1280 : 768)) s = 1;
+            if (groups > 0) least = 32768;   // what sequences have of their own behind a shared prefix is taken to be short
+        } else if (tile <= 32) {
+            least = 4 * tile;   // 9 sequences on 480 shared keys: 13.5 us in pieces of 64, 17 in ones of 256
+            const int64_t most = keys / 512 > 16 ? keys / 512 : 16;   // those behind wait for the sums: 16 sequences on 2048, one key head, in 16 pieces 16 us, in 32 18
+            s = s < most ? s : most;
+        }
         s = s < (keys + least - 1) / least ? s : (keys + least - 1) / least;
         splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
     };
@@ -1215,12 +1160,6 @@ AttnPlan quant_attention_plan(int T, int B, bool single, int groups, int hq, int
     if (single) p.own_tiles = (int64_t)T * ((hq / heads + p.own_rows - 1) / p.own_rows);
     if (groups > 0) side(groups, false, p.group_rows, p.group_tiles, p.group_splits);
     p.slots = p.own_splits + p.group_splits;
-    // few sequences of one token each, whose lengths decide how long the card is busy: pieces of one size
-    if (single && groups == 0 && B >= 16 && B <= 256 && p.own_rows >= hq / heads && p.own_splits > 1) {
-        p.share = (int)((1024 + heads - 1) / heads);
-        p.slots = p.own_splits * 4 < 64 ? p.own_splits * 4 : 64;
-        p.own_tiles = p.share + B + (T - B);
-    }
     return p;
 }
 
@@ -1230,18 +1169,16 @@ void launch_quant_attention(int kind, int D, const AttnPlan& p, const uint16_t* 
     if (T == 0) return;
     AttnArgs a{q, q_stride, cache, bt, bt_stride, width, q_start, ctx_len, groups ? group_start : nullptr, prefix_len, B, T, groups, hq, scale * 1.4426950408889634f,
                out, part_o, part_l, p.slots, 0, 0,
-               (cache.page & (cache.page - 1)) ? -1 : __builtin_ctz(cache.page), false, false, 0};
+               (cache.page & (cache.page - 1)) ? -1 : __builtin_ctz(cache.page), false, false};
     if (groups) {
         a.splits = p.group_splits;
         a.slot0 = 0;
         launch_rows_of<true>(kind, D, p.group_rows, a, p.group_tiles, st);
     }
-    a.splits = p.share ? 1 : p.own_splits;
-    a.share = p.share;
+    a.splits = p.own_splits;
     a.slot0 = p.group_splits;
     a.last = groups && p.own_rows <= 32 && p.own_splits == 1;
-    // tiles of 256 rows have a CU each, of 128 half of one
-    a.longest = q_start && !groups && B < 256 && p.own_rows > 32 && p.own_tiles * cache.heads > (p.own_rows == 256 ? 256 : 512);
+    a.longest = q_start && !groups && B < 256 && p.own_rows == 256 && p.own_tiles * cache.heads > 256;   // a tile has a CU for itself
     launch_rows_of<false>(kind, D, p.own_rows, a, p.own_tiles, st);
     if (p.slots > 1 && !a.last) {
         const int64_t rows = (int64_t)T * hq;

@@ -90,6 +90,27 @@ def test_attention(case):
     assert torch.equal(out, ops.quant_attention(q, cache, table, ctx, q_start))
 
 
+# the other forms that the rules choose, by heads rather than rows
+FORMS = [
+    ("mxfp4", 64, 64, 64, 16, [800, 31], [300, 30]),            # tiles of 256 rows, the keys in two pieces
+    ("int8", 128, 32, 32, 16, [900], [900]),
+    ("int8", 64, 64, 64, 32, [700], [600]),                     # in one
+    ("int8", 128, 16, 8, 16, [5000] + [37 * i % 300 for i in range(20)], None),             # pieces of one size
+    ("mxfp4", 64, 8, 4, 16, [4100] + [1 + 91 * i % 1300 for i in range(39)], None),
+    ("int8", 128, 8, 1, 64, [300] * 140 + [17000, 0, 9000], None),
+    ("int8", 64, 16, 8, 64, [4100] + [100 + i for i in range(29)], [1 + i % 2 for i in range(30)]),      # two pieces
+    ("mxfp4", 128, 16, 8, 32, [500] * 28, [9 + i % 3 for i in range(28)]),                  # 32 rows
+]
+
+
+@pytest.mark.parametrize("case", FORMS, ids=lambda c: "-".join(map(str, c[:5])) + f"-{max(c[5])}-{len(c[5])}")
+def test_forms(case):
+    q, cache, table, ctx, q_start = t.attention_case(*case, DEV, tail=3)
+    out = ops.quant_attention(q, cache, table, ctx, q_start)
+    t.check_attention(out, q, cpu(cache), table, ctx.cpu(), None if q_start is None else q_start.cpu())
+    assert not out[-3:].any()
+
+
 # more tiles than the card holds at a time, which go by their lengths: (kind, D, hq, hkv, page, contexts, tokens, keys that the table has room for)
 LONGEST = [
     ("int8", 64, 64, 64, 16, [300, 0, 517, 129, 64, 700], [300, 0, 260, 129, 5, 600], 0),
@@ -183,6 +204,22 @@ def test_prefix(case):
     assert torch.equal(out, ops.prefix_attention(q, cache, table, ctx, groups, prefix + case[4] - 1, q_start))    # whole pages only
     alone = ops.prefix_attention(q, cache, table, ctx, groups[:1], prefix[:0], q_start)                           # no groups
     assert torch.equal(alone, ops.quant_attention(q, cache, table, ctx, q_start))
+
+
+PREFIX_FORMS = [
+    ("int8", 128, 32, 16, 16, [40], [100], [1 + i % 29 for i in range(100)], None, 1),      # tiles of 128 rows
+    ("mxfp4", 64, 64, 32, 16, [40], [60], [1 + i % 29 for i in range(60)], None, 2),        # of 256
+    ("int8", 64, 64, 32, 32, [9, 20], [40, 30], [3 + i % 29 for i in range(70)], [1 + i % 3 for i in range(70)], 0),
+    ("mxfp4", 128, 32, 8, 16, [50], [40], [1 + i % 29 for i in range(40)], None, 0),        # of 32
+    ("int8", 64, 64, 64, 16, [3], [3], [200, 160, 170], [150, 150, 160], 1),                # the own keys' of 256
+]
+
+
+@pytest.mark.parametrize("case", PREFIX_FORMS, ids=lambda c: "-".join(map(str, c[:5])) + f"-{max(c[5])}-{len(c[7])}")
+def test_prefix_forms(case):
+    (q, table, ctx, groups, prefix, q_start), cache = prefix_case(*case)
+    out = ops.prefix_attention(q, cache, table, ctx, groups, prefix, q_start)
+    t.check_attention(out, q, cpu(cache), table, ctx.cpu(), None if q_start is None else q_start.cpu())
 
 
 @pytest.mark.parametrize("kind", t.KINDS)
