@@ -4,14 +4,14 @@
 //   out_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i . k_j - m_i),  over the keys j <= position of i; token i of a sequence is at ctx - len + i.
 //
 // Rows are (token, query head) pairs of one key head; a workgroup takes a tile of 16 NQT rows, of one sequence, one key head and one piece of the keys.  Its four
-// waves take steps of 32 keys in turn, each with a running maximum and sum, and are joined through LDS; pieces of the keys are joined by a second launch.  S^T = K Q^T
+// waves take steps of 32 keys in turn, each with a running reference and sum, and are joined through LDS; pieces of the keys are joined by a second launch.  S^T = K Q^T
 // and O^T = V^T P^T on v_mfma_f32_16x16x32_bf16: with the keys as rows of the first product a lane holds the scores of its own query row, and the probabilities are
 // the second one's operand as they are.  Codes go from memory to registers and become bfloat16 there, which is exact (eight bits, and e2m1 times a power of two):
 //   * K: the dimensions of a product may be taken in any order that queries and keys share, so a lane takes its row's bytes 16 at a time;
 //   * V: the operand wants eight keys of one dimension, the page has the dimensions of one key.  Row m of product dt is dimension m D / 16 + dt: a lane then needs the
 //     same D / 16 neighbouring bytes of its eight keys, for all products, and no exchange between lanes.
-// int8: a key's scale multiplies its scores, a value's the probabilities.  These are then rounded to float16 (2^-12): in bfloat16 the largest probability of a row, 1 times a scale, would
-// be off by up to 2^-9 where without scales it is exact (.0025 of the output's size in place of .0017, of which its own rounding is .0016).  Each row's sums have a reference
+// int8: a key's scale multiplies its scores, a value's the probabilities.  These are then rounded to float16 (2^-11): in bfloat16 the largest probability of a row, 1 times a scale, would
+// be off by up to 2^-8 where without scales it is exact (.0025 of the output's size in place of .0017, of which its own rounding is .0016).  Each row's sums have a reference
 // that keeps its products in float16's range, the largest at 2^7 to 2^15, whatever the scales are; what is 2^-32 of the largest and less may get lost.  mxfp4: the conversion takes the scale, probabilities are bfloat16.
 //
 // The reference that a row's probabilities are 2^(score - ref) of only moves when a score is far over it (2^8; int8: as float16 allows): rescaling the sums costs as much as all
@@ -412,6 +412,8 @@ template <int N> __device__ __forceinline__ float moved_ref(float& ref, float ba
 // ---- the tile -----------------------------------------------------------------------------------------------------------------------------------------
 // GROUPS: the items are groups of sequences, the keys those that each shares; otherwise sequences, their keys behind what they share.
 // ONCE: the codes are marked as read once.
+// Bound by the codes' bytes where keys are many (two sequences of 128k, 64 query heads, mxfp4: 285 MB in 55 us, 5.2 TB/s; the join behind it 5), by the chain of loads (length, page, codes)
+// and the waves' join where they are few (a sequence of 140 keys 6.8 us).
 template <int KIND, int D, int NQT, bool GROUPS, bool ONCE>
 __global__ void __launch_bounds__(256, NQT == 1 ? (KIND == kInt8 && D == 128 ? 3 : 4) : 2) quant_rows_kernel(const AttnArgs a) {
     constexpr int ROWS = 16 * NQT, NC = D / 32, ND = D / 16;
@@ -678,6 +680,9 @@ __global__ void __launch_bounds__(256, NQT == 1 ? (KIND == kInt8 && D == 128 ? 3
 // loaded a step earlier, into the buffer that is not being read; one barrier a step.  16 bytes behind every row keep its readers, 16 bytes a lane and a row
 // each, out of each other's banks.  v_mfma_f32_32x32x16: a lane has 16 of 32 keys of one row, and the probabilities are the second product's operand as they are, its values' keys in the same order
 // (4 h + (j & 3) + 8 (j >> 2) of 16).
+// Two prompts of 1950 tokens and two of 330 on up to 3296 keys, 32 query heads, int8, 113 GFLOP: 174 us, 650 TFLOP/s; 2 x 128 sequences of 64 query heads on 16k shared keys, mxfp4,
+// 137 GFLOP: 150 us, 920 TFLOP/s.  There matrix cores are busy 39 % of the time and vector ALUs 44 %, one after the other for the most part: priorities of waves, half of them a step's part
+// late, products a part late beside the next probabilities (which spills), and reads from LDS further ahead all gain nothing or lose.
 template <int KIND, int D, int WAVES> struct TileStep {
     static constexpr int KT = 16 * WAVES, KS = 2 * D + 16, VS = 2 * KT + 16;   // bytes from key to key, and from dimension to dimension
     alignas(16) uint8_t k[KT * KS];
@@ -1080,6 +1085,9 @@ __global__ void __launch_bounds__(256) quant_join_kernel(const float* __restrict
 }
 
 template <int KIND, int D, bool GROUPS> void launch_rows(int rows, const AttnArgs& a, int64_t tiles, hipStream_t st) {
+    // Marked as read once from 192 MiB of codes on (by the table's width).  Where caches are many, a layer each, that gains 3 to 7 % (int8, 64 sequences of 2048, 256 MiB: 52 and 48 us;
+    // mxfp4, two of 128k: 63 and 60); where the last cache (256 MB) still holds this one from the call before, it loses (64 of 2048: 45 and 49; mxfp4, 80 of 2048, 160 MiB: 35 and 39), and so
+    // smaller ones are not.
     const bool once = !a.group_start && (int64_t)a.B * a.width * a.cache.page * a.cache.heads * row_bytes<KIND, D>() * 2 >= (int64_t)192 << 20;
     const dim3 g((unsigned)(tiles * a.cache.heads), a.splits), b(256);
     if (rows == 16) {
@@ -1178,7 +1186,8 @@ void launch_quant_attention(int kind, int D, const AttnPlan& p, const uint16_t* 
     a.splits = p.own_splits;
     a.slot0 = p.group_splits;
     a.last = groups && p.own_rows <= 32 && p.own_splits == 1;
-    a.longest = q_start && !groups && B < 256 && p.own_rows == 256 && p.own_tiles * cache.heads > 256;   // a tile has a CU for itself
+    // A tile of 256 rows has a CU for itself.  Prompts of up to 2048 tokens behind up to 2048 of context, two of them: 163 us so, 218 in order; 16 of up to 256: 64 and 66.
+    a.longest = q_start && !groups && B < 256 && p.own_rows == 256 && p.own_tiles * cache.heads > 256;
     launch_rows_of<false>(kind, D, p.own_rows, a, p.own_tiles, st);
     if (p.slots > 1 && !a.last) {
         const int64_t rows = (int64_t)T * hq;
