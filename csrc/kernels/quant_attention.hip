@@ -1115,21 +1115,21 @@ template <bool GROUPS> void launch_rows_of(int kind, int D, int rows, const Attn
 }
 
 // workgroups of a launch with tiles of `tile` rows, without pieces, if the items' rows are alike
-int64_t groups_of(int64_t rows, int64_t items, int heads, int tile) {
+int64_t workgroups(int64_t rows, int64_t items, int heads, int tile) {
     const int64_t tiles = (rows + tile - 1) / tile;
     return (tiles > items ? tiles : items) * heads;
 }
 // Rows of a tile, by the rows that an item has on average and the workgroups that this makes.  Small tiles read the keys more often, and large ones leave CUs idle and rows
-// empty.  Sequences (32 query and 8 key heads of 128, int8; 16 / 32 / 128 / 256 rows): 8 x 64 rows on 2000 keys 25 / 31 / 69 / 56 us; 32 x 64 on 2000 65 / 46 / 94 / 76;
-// 32 x 128 on 2000 112 / 82 / 96 / 77; 4 x 512 on 500 24 / 18 / 27 / 28.  What a group shares (4 rows a sequence and key head): 16 sequences on 2048 keys 20 / 21 / 26 / 27,
-// 64 on 8192 48 / 38 / 50 / 45, 128 on 16384 - / 107 / 92 / 112, two groups of those - / - / 149 / 130.
+// empty.  16 / 32 / 128 / 256 rows, each with the pieces that suit it best, 32 query and 8 key heads of 128, int8: 8 sequences of 64 rows on 2000 keys 25 / 27 / 33 / 33 us, 32 of 64 on 2000
+// 65 / 46 / 69 / 76, 32 of 128 on 2000 112 / 82 / 96 / 77, 32 of 128 on 500 41 / 33 / 34 / 31, 4 of 512 on 500 24 / 18 / 27 / 28.  What a group shares (4 rows a sequence and key head):
+// 16 sequences on 2048 keys 20 / 21 / 24 / 24, 64 on 8192 53 / 38 / 50 / 45, 128 on 16384 139 / 107 / 92 / 112, two groups of those 259 / 194 / 149 / 130.
 int tile_of(int64_t rows, int64_t items, int heads, int64_t keys, bool own) {
     const int64_t per = items > 0 ? rows / items : rows;
     if (per <= 16) return 16;
     // 1 x 128 rows on 16000 keys: 43 us in 16 pieces with 16 rows, 34 with 32; 2 x 64 sequences of 8 rows on 8192, one key head: 37 and 30
-    if (groups_of(rows, items, heads, 16) <= (own ? 256 : 64) && (own ? per <= 64 || keys < 4096 : per <= 128)) return 16;
-    if (per >= 112 && groups_of(rows, items, heads, 256) >= (own ? 128 : 32)) return 256;
-    return !own && per >= 192 && groups_of(rows, items, heads, 256) >= 16 ? 128 : 32;
+    if (workgroups(rows, items, heads, 16) <= (own ? 256 : 64) && (own ? per <= 64 || keys < 4096 : per <= 128)) return 16;
+    if (per >= 112 && workgroups(rows, items, heads, 256) >= (own ? 128 : 32)) return 256;
+    return !own && per >= 192 && workgroups(rows, items, heads, 256) >= 16 ? 128 : 32;
 }
 
 }  // namespace
@@ -1141,7 +1141,7 @@ AttnPlan quant_attention_plan(int T, int B, bool single, int groups, int hq, int
     auto side = [&](int64_t items, bool own, int& tile, int64_t& tiles, int& splits) {
         tile = tile_of(rows, items, heads, keys, own);
         tiles = rows / tile + items + 1;
-        const int64_t wgs = groups_of(rows, items, heads, tile), full = tile == 256 ? 256 : 512;   // a workgroup a CU, or two
+        const int64_t wgs = workgroups(rows, items, heads, tile), full = tile == 256 ? 256 : 512;   // a workgroup a CU, or two
         int64_t s = full / wgs, least = 256;
         if (own) {
             const int64_t busy = rows > 16 * items ? 160 : 224;

@@ -75,7 +75,7 @@ MORE = [
     ("int8", 128, 8, 1, 16, [2100], [40]),                      # tiles of 256 rows
     ("mxfp4", 64, 16, 2, 32, [2050, 2100], [35, 33]),
     ("int8", 64, 16, 1, 16, [2049], [20]),
-    ("int8", 128, 8, 2, 16, [1 + 97 * i % 1500 for i in range(20)] + [0, 1500], None),      # pieces of one size
+    ("int8", 128, 8, 2, 16, [1 + 97 * i % 1500 for i in range(20)] + [0, 1500], None),      # lengths far apart
     ("mxfp4", 64, 8, 4, 16, [(31 * i * i) % 700 for i in range(150)], None),
     ("mxfp4", 128, 16, 2, 64, [20] * 30 + [3000], None),
 ]
@@ -95,7 +95,7 @@ FORMS = [
     ("mxfp4", 64, 64, 64, 16, [800, 31], [300, 30]),            # tiles of 256 rows, the keys in two pieces
     ("int8", 128, 32, 32, 16, [900], [900]),
     ("int8", 64, 64, 64, 32, [700], [600]),                     # in one
-    ("int8", 128, 16, 8, 16, [5000] + [37 * i % 300 for i in range(20)], None),             # pieces of one size
+    ("int8", 128, 16, 8, 16, [5000] + [37 * i % 300 for i in range(20)], None),             # lengths far apart
     ("mxfp4", 64, 8, 4, 16, [4100] + [1 + 91 * i % 1300 for i in range(39)], None),
     ("int8", 128, 8, 1, 64, [300] * 140 + [17000, 0, 9000], None),
     ("int8", 64, 16, 8, 64, [4100] + [100 + i for i in range(29)], [1 + i % 2 for i in range(30)]),      # two pieces
