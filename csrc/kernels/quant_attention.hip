@@ -15,7 +15,8 @@
 // that keeps its products in float16's range, the largest at 2^7 to 2^15, whatever the scales are; what is 2^-32 of the largest and less may get lost.  mxfp4: the conversion takes the scale, probabilities are bfloat16.
 //
 // The reference that a row's probabilities are 2^(score - ref) of only moves when a score is far over it (2^8; int8: as float16 allows): rescaling the sums costs as much as all
-// else that a step does to them, and while it stays no lane needs to know of another.
+// else that a step does to them, and while it stays no lane needs to know of another.  mxfp4: where values are so large that 2^8 times as much, over 2^30 keys, would pass float32's
+// range (E over 213, numbers over 2^86), the scores stay as far below the reference as it takes (most_over).  Averages are joined with weights that add up to one, or 2^-8 of them.
 //
 // What no sum may take: keys behind the position, behind the context, on pages that the table does not have (numbers outside 0 .. pages - 1 are left out): their
 // scores are -inf and their probabilities zero by selection, not by product; their values cannot be NaN either (a value scale of NaN acts on the probabilities of
@@ -398,6 +399,8 @@ template <int KIND> __device__ __forceinline__ uint32_t round2(float a, float b)
     else return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
 }
 
+// mxfp4: how far scores over the reference may be beside values of exponents up to E (bytes of the cache, 252 at most).  A value is less than 2^(E - 124), so 2^30 products stay within 2^127.
+__device__ __forceinline__ float most_over(uint32_t E) { return fminf(8.f, 221.f - (float)E); }
 // A row's reference moves: to `up` over base, the highest score so far or (int8) what its probabilities times scales allow; never down, once there is one.  x are the
 // scores over base, and then over the new one; returns what sums so far are to be multiplied by.
 template <int N> __device__ __forceinline__ float moved_ref(float& ref, float base, float mx, float up, float (&x)[N]) {
@@ -493,9 +496,10 @@ __global__ void __launch_bounds__(256, NQT == 1 ? (KIND == kInt8 && D == 128 ? 3
                 for (int qt = 0; qt < NQT; ++qt) sc[qt][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[qt][c], sc[qt][g], 0, 0, 0);
             }
         }
-        // Values that are NaN, by their scales: 4-bit ones from 253 on (192 and more does not come from numbers: looked for in all keys at once), float ones that are
+        // Values that are NaN, by their scales: 4-bit ones from 253 on (192 and more, which is 2^65, is looked for in all keys at once), float ones that are
         // not finite (or negative).  They count as zeros and their keys' scores as NaN.
         uint32_t nan = 0, top = 0;   // of this lane's keys, bit j; int8: the largest scale's bits
+        float over = 8.f;            // mxfp4: most_over of this lane's keys
         if constexpr (KIND == kFp4) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) top |= s.ve[j] & (s.ve[j] << 1) & 0x80808080u;
@@ -509,11 +513,15 @@ __global__ void __launch_bounds__(256, NQT == 1 ? (KIND == kInt8 && D == 128 ? 3
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
 #pragma unroll
-                    for (int b = 0; b < D / 32; ++b)
-                        if (((s.ve[j] >> (8 * b)) & 255) > 252) {
+                    for (int b = 0; b < D / 32; ++b) {
+                        const uint32_t E = (s.ve[j] >> (8 * b)) & 255;
+                        if (E > 252) {
                             nan |= 1u << j;
                             s.ve[j] &= ~(255u << (8 * b));
+                        } else {
+                            over = fminf(over, most_over(E));
                         }
+                    }
             } else {
                 top = 0;
 #pragma unroll
@@ -527,7 +535,7 @@ __global__ void __launch_bounds__(256, NQT == 1 ? (KIND == kInt8 && D == 128 ? 3
         }
         const bool part = odd || t0 + 32 > ke || t0 + 31 > first || s.blk[0] < 0 || s.blk[1] < 0;   // some row does not see some key
         // scores over the reference may be so high: int8, times the lane's scales, as float16 holds
-        const float most = KIND == kInt8 ? fminf(15.f - __log2f(__uint_as_float(top)), 100.f) : 8.f;
+        const float most = KIND == kInt8 ? fminf(15.f - __log2f(__uint_as_float(top)), 100.f) : over;
         uint4 pw[NQT];
 #pragma unroll
         for (int qt = 0; qt < NQT; ++qt) {
@@ -549,8 +557,8 @@ __global__ void __launch_bounds__(256, NQT == 1 ? (KIND == kInt8 && D == 128 ? 3
 #pragma unroll
             for (int j = 0; j < 8; ++j) mx = fmaxf(mx, x[j]);
             if (__builtin_expect(__ballot(mx > (ref[qt] == -INFINITY ? -INFINITY : most)) != 0, false)) {
+                float up = rows_max(mx - fminf(most, 0.f));   // mxfp4
                 mx = rows_max(mx);
-                float up = mx;
                 if constexpr (KIND == kInt8) {
                     up = -INFINITY;
 #pragma unroll
@@ -614,12 +622,15 @@ __global__ void __launch_bounds__(256, NQT == 1 ? (KIND == kInt8 && D == 128 ? 3
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
                         for (int c = 0; c < ND / 4; ++c) x[i][c] = *reinterpret_cast<const f32x4*>(a.part_o + at * D + (4 * h4 + i) * ND + 4 * c);
-                    const float mx = fmaxf(lse, other), f = __builtin_amdgcn_exp2f(lse - mx), g = __builtin_amdgcn_exp2f(other - mx), both = 1.f / (f + g);
+                    const float mx = fmaxf(lse, other);
+                    float f = __builtin_amdgcn_exp2f(lse - mx), g = __builtin_amdgcn_exp2f(other - mx);
+                    const float both = 1.f / (f + g);
                     lse = mx + __log2f(f + g);
+                    f *= both, g *= both;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int dt = 0; dt < ND; ++dt) o[qt][dt][i] = (o[qt][dt][i] * f + x[i][dt >> 2][dt & 3] * g) * both;
+                        for (int dt = 0; dt < ND; ++dt) o[qt][dt][i] = o[qt][dt][i] * f + x[i][dt >> 2][dt & 3] * g;
                 }
             }
         }
@@ -637,24 +648,26 @@ __global__ void __launch_bounds__(256, NQT == 1 ? (KIND == kInt8 && D == 128 ? 3
 #pragma unroll
             for (int p = 0; p < 3; ++p) mx = fmaxf(mx, sl[p][lane]);
             const float base = mx == -INFINITY ? 0.f : mx;
-            float f = __builtin_amdgcn_exp2f(lse - base), sum = f;
+            float f = __builtin_amdgcn_exp2f(lse - base), g[3], sum = f;
+#pragma unroll
+            for (int p = 0; p < 3; ++p) sum += g[p] = __builtin_amdgcn_exp2f(sl[p][lane] - base);
+            const float one = sum == 0.f ? 0.f : 1.f / sum;
+            f *= one;
 #pragma unroll
             for (int dt = 0; dt < ND; ++dt) o[qt][dt] *= f;
 #pragma unroll
             for (int p = 0; p < 3; ++p) {
-                f = __builtin_amdgcn_exp2f(sl[p][lane] - base);
-                sum += f;
+                g[p] *= one;
 #pragma unroll
-                for (int dt = 0; dt < ND; ++dt) o[qt][dt] += so[p][dt][lane] * f;
+                for (int dt = 0; dt < ND; ++dt) o[qt][dt] += so[p][dt][lane] * g[p];
             }
-            const float one = sum == 0.f ? 0.f : 1.f / sum;
             if (live && (a.slots == 1 || a.last)) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint16_t* dst = a.out + row * D + (4 * h4 + i) * ND;
                     uint16_t v[ND];
 #pragma unroll
-                    for (int dt = 0; dt < ND; ++dt) v[dt] = f2bf(o[qt][dt][i] * one);
+                    for (int dt = 0; dt < ND; ++dt) v[dt] = f2bf(o[qt][dt][i]);
                     if constexpr (ND == 8) *reinterpret_cast<u16x8*>(dst) = u16x8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
                     else *reinterpret_cast<u16x4*>(dst) = u16x4{v[0], v[1], v[2], v[3]};
                 }
@@ -667,7 +680,7 @@ __global__ void __launch_bounds__(256, NQT == 1 ? (KIND == kInt8 && D == 128 ? 3
 #pragma unroll
                         for (int dt = 0; dt < ND; dt += 4)
                             *reinterpret_cast<f32x4*>(a.part_o + at * D + (4 * h4 + i) * ND + dt) =
-                                f32x4{o[qt][dt][i], o[qt][dt + 1][i], o[qt][dt + 2][i], o[qt][dt + 3][i]} * one;
+                                f32x4{o[qt][dt][i], o[qt][dt + 1][i], o[qt][dt + 2][i], o[qt][dt + 3][i]};
                 }
             }
         }
@@ -689,7 +702,7 @@ template <int KIND, int D, int WAVES> struct TileStep {
     alignas(16) uint8_t v[D * VS];
     alignas(16) float km[KT], vm[KT];   // int8: scales of keys, times scale_log2, and values; 0 where a key is not there
     uint32_t there[KT / 32], nan[KT / 32];
-    float top[KT / 32];                 // int8: base-2 logarithm of the largest of vm
+    float top[KT / 32];                 // int8: base-2 logarithm of the largest of vm; mxfp4: most_over of the values
 };
 
 // 32 keys' codes on their way into LDS, by one wave: keys or values
@@ -774,7 +787,16 @@ template <int KIND, int D> struct Fetch {
 #pragma unroll
             for (int b = 0; b < D / 32; ++b) bad |= (scale >> (8 * b) & 255) > 252;
             const uint32_t nan = (uint32_t)__ballot(bad && here && lane < 32);
-            if (lane == 0) s.there[i] = there, s.nan[i] = nan;
+            float over = 8.f;
+            if (__ballot(scale & (scale << 1) & 0x80808080u)) {   // values from 2^65 on (D = 64: `scale` has two bytes)
+#pragma unroll
+                for (int b = 0; b < D / 32; ++b) {
+                    const uint32_t E = scale >> (8 * b) & 255;
+                    if (here && E <= 252) over = fminf(over, most_over(E));
+                }
+                over = -wave_max(-over);
+            }
+            if (lane == 0) s.there[i] = there, s.nan[i] = nan, s.top[i] = over;
         }
         constexpr int KP = 1024 / RB;
 #pragma unroll
@@ -920,10 +942,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[i]);
         // scores over the reference may be so high: int8, times the largest scale, as float16 holds
-        const float most = KIND == kInt8 ? fminf(15.f - s.top[sub], 100.f) : 8.f;
+        const float most = KIND == kInt8 ? fminf(15.f - s.top[sub], 100.f) : s.top[sub];
         if (__builtin_expect(__ballot(mx > (ref == -INFINITY ? -INFINITY : most)) != 0, false)) {
             mx = lanes_xor32(mx, LaneMax{});
-            float up = mx;
+            float up = mx - fminf(most, 0.f);   // mxfp4
             if constexpr (KIND == kInt8) {
                 up = -INFINITY;
 #pragma unroll
@@ -1025,7 +1047,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) quant_tile_kernel(const AttnArg
 }
 
 // Rows of the pieces' averages o_s, of sums 2^(l_s): out = sum_s 2^(l_s - m) o_s / sum_s 2^(l_s - m).  D / 4 lanes have a row, `per` such groups share its pieces and are
-// joined through LDS.  The sums of up to D / 4 pieces are read at once, a lane each, and handed round; what the pieces hold does not wait for them.
+// joined through LDS.  Weights are 2^-8 of what they are: those of up to 128 pieces then add up to no more than a half, so that averages near the end of float32's range keep within it.
+// The sums of up to D / 4 pieces are read at once, a lane each, and handed round; what the pieces hold does not wait for them.
 template <int D>
 __global__ void __launch_bounds__(256) quant_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_l, uint16_t* __restrict__ out, int64_t rows,
                                                          int slots, int per) {
@@ -1058,7 +1081,7 @@ __global__ void __launch_bounds__(256) quant_join_kernel(const float* __restrict
 #pragma unroll 4
         for (int i = 0; i < upto; ++i, p += per * rows * D) {
             const f32x4 x = *reinterpret_cast<const f32x4*>(p);
-            const float f = __shfl(w, i, L);
+            const float f = __shfl(w, i, L) * 0x1p-8f;
             const bool on = __shfl((int)there, i, L);   // what an empty piece has there was never written
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[j] += on ? x[j] * f : 0.f;
@@ -1080,7 +1103,7 @@ __global__ void __launch_bounds__(256) quant_join_kernel(const float* __restrict
         }
     }
     if (at >= rows) return;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const float inv = sum == 0.f ? 0.f : 0x1p8f / sum;
     *reinterpret_cast<u16x4*>(out + row * D + 4 * c) = u16x4{f2bf(o[0] * inv), f2bf(o[1] * inv), f2bf(o[2] * inv), f2bf(o[3] * inv)};
 }
 

@@ -101,6 +101,6 @@ def quant_attention(q, cache, block_table, ctx_len, q_start, scale):
         p = torch.exp(s - torch.where(top == float("-inf"), 0.0, top))
         p = torch.where(seen & bad[:, None, None], float("nan"), p)
         l = p.sum(-1, keepdim=True)
-        o = torch.where(l == 0, 0.0, (p @ v[:, None]) / l)
+        o = torch.where(l == 0, 0.0, (p / l) @ v[:, None])                 # no sum is larger than the largest value
         out[start[b]:start[b + 1]] = o.permute(2, 0, 1, 3).reshape(n, hq, D).to(q.dtype)
     return out

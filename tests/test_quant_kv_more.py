@@ -1,0 +1,56 @@
+"""A key/value cache in 8 or 4 bits: the ends of its ranges and what its documentation allows, on the CPU.  The kernels' tests (test_quant_kv_more_gpu.py) take their cases from here."""
+import pytest
+import torch
+
+from chronos import ops
+from tests import test_quant_kv as t
+from tests.oracles import quant_kv_plain as plain
+from tests.oracles import quant_kv_whole as whole
+
+BF = torch.bfloat16
+
+
+def check(out, q, cache, table, ctx, q_start=None, more=0.0):
+    """:func:`test_quant_kv.check_attention`'s bound, against the oracle for many rows; ``more``: what else is off relative to sum_j p_j |v_j|."""
+    want, size = whole.attention(q, cache, table, ctx, q_start)
+    want, size = want.cpu(), size.cpu()
+    off, most = (out.double().cpu() - want).abs(), t.HALF * want.abs() + (t.HALF + 2 ** -10 + more) * size + 1e-30
+    assert torch.equal(torch.isnan(out.cpu()), torch.isnan(want))
+    worst = torch.nan_to_num(off / most, nan=0.0).max() if off.numel() else 0.0
+    assert worst <= 1, f"{float(worst)} of what roundings allow"
+
+
+@pytest.mark.parametrize("case", t.ATTENTION, ids=lambda c: "-".join(map(str, c[:5])) + f"-{len(c[5])}")
+def test_the_oracles_agree(case):
+    q, cache, table, ctx, q_start = t.attention_case(*case, tail=2)
+    cache.vs[int(table[0, 0]), 0, 0] = float("nan") if case[0] == "int8" else 255
+    table[-1, 0] = -1
+    for a, b in zip(plain.attention(q, cache, table, ctx, q_start), whole.attention(q, cache, table, ctx, q_start)):
+        assert torch.allclose(a, b, rtol=1e-12, atol=1e-14, equal_nan=True)
+
+
+def loud_values(cache, table, rising):
+    """mxfp4 values up to the format's end, 6 2^125.  rising: exponents from 2^73 up to there, key by key, and keys that grow with their pages' places."""
+    if not rising:
+        cache.vs.fill_(252)
+        return
+    at = torch.arange(cache.vs[..., 0].numel(), device=cache.vs.device).view(cache.vs.shape[:-1])
+    cache.vs.copy_((200 + (at * 37) % 53)[..., None].expand(cache.vs.shape))
+    for p, i in {p: i for row in table.tolist() for i, p in enumerate(row) if i}.items():      # a shared page once
+        cache.ks[p] += min(4, i // 6)
+
+
+def check_loud(q, cache, table, ctx, q_start, attend):
+    """Averages of values near the end of float32's range are finite, as sums of them are not."""
+    loud_values(cache, table, False)
+    check(attend(q * 0), q * 0, cache, table, ctx, q_start)
+    check(attend(q), q, cache, table, ctx, q_start)
+    loud_values(cache, table, True)
+    q = q / 16                                                   # keys are up to 16 times as large
+    check(attend(q), q, cache, table, ctx, q_start)
+
+
+@pytest.mark.parametrize("lens", (None, [40, 130]), ids=("rows", "prompts"))
+def test_values_at_the_end_of_the_range(lens):
+    q, cache, table, ctx, q_start = t.attention_case("mxfp4", 64, 4, 2, 16, [120, 333], lens)
+    check_loud(q, cache, table, ctx, q_start, lambda x: ops.quant_attention(x, cache, table, ctx, q_start))
