@@ -7,7 +7,8 @@
 //           A number is its code's value (0 .5 1 1.5 2 3 4 6, the top bit the sign) times 2^(E - 127), one E per 32 dimensions: the smallest with
 //           max|x| <= 7 2^(E - 127), in 1 .. 252 (larger maxima are cut off at 6 2^125).  Up to 7 and not to 6, as 6 is the nearest code up to there: over normal
 //           values the error is .112 of their size, .115 with 6 or 8 in its place.
-//   A row (token, head) that holds an infinity or a NaN is held as NaN as a whole: scale NaN, E = 255 in all its blocks.
+//   A row (token, head) that holds an infinity or a NaN is held as NaN as a whole: scale NaN, E = 255 in all its blocks.  253 and 254, which no write makes, are read as 255
+//   is: six of their units pass float32's range.
 #pragma once
 #include "chronos_hip.h"
 
@@ -36,6 +37,9 @@ template <int KIND, int D> constexpr int scale_bytes() { return KIND == kInt8 ? 
 __device__ __forceinline__ float code8(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// the power of two that E stands for
+__device__ __forceinline__ float unit4(uint32_t E) { return __uint_as_float((E > 252 ? 255 : E) << 23); }
 
 // bfloat16 of the eight e2m1 codes of a word, times a power of two (exact)
 __device__ __forceinline__ void codes4(uint32_t w, float scale, bf16x2 (&v)[4]) {

@@ -337,7 +337,7 @@ template <int KIND, int D> __device__ __forceinline__ bf16x8 key_operand(const S
         return eight(s.k[g][2 * c], s.k[g][2 * c + 1]);
     } else {
         bf16x2 b[4];
-        codes4(s.k[g][c], __uint_as_float(s.ke[g] << 23), b);
+        codes4(s.k[g][c], unit4(s.ke[g]), b);
         return bf16x8{b[0][0], b[0][1], b[1][0], b[1][1], b[2][0], b[2][1], b[3][0], b[3][1]};
     }
 }
@@ -809,7 +809,7 @@ template <int KIND, int D> struct Fetch {
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     bf16x2 b[4];
-                    codes4(w[4 * p + x], __uint_as_float(e[p] << 23), b);
+                    codes4(w[4 * p + x], unit4(e[p]), b);
                     *reinterpret_cast<bf16x8*>(s.k + at * s.KS + (4 * part + x) * 16) = bf16x8{b[0][0], b[0][1], b[1][0], b[1][1], b[2][0], b[2][1], b[3][0], b[3][1]};
                 }
             }

@@ -244,9 +244,9 @@ __global__ void __launch_bounds__(256) quant_kv_read_kernel(const int32_t* __res
                 for (int j = 0; j < 8; ++j) o[j] = f2bf(code8(w[kv][i][j >> 2], j & 3) * s);
             } else {
                 bf16x2 b[4];
-                codes4(w[kv][i][0], __uint_as_float(e[kv][i] << 23), b);
+                codes4(w[kv][i][0], unit4(e[kv][i]), b);
                 o = __builtin_bit_cast(u16x8, (bf16x8{b[0][0], b[0][1], b[1][0], b[1][1], b[2][0], b[2][1], b[3][0], b[3][1]}));
-                if (e[kv][i] == 255) o = u16x8{0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0};
+                if (e[kv][i] > 252) o = u16x8{0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0, 0x7fc0};
             }
             if (!there[i]) o = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
             *reinterpret_cast<u16x8*>((kv ? v : k) + (first + S * i) * D + 8 * c) = o;

@@ -32,7 +32,7 @@ def decode(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
         return codes.float() * scales[..., None]
     grid = torch.tensor(E2M1 + tuple(-x for x in E2M1), device=codes.device)
     x = grid[torch.stack([codes & 15, codes >> 4], -1).flatten(-2).long()].unflatten(-1, (-1, 32))
-    s = torch.where(scales == 255, float("nan"), torch.ldexp(torch.ones((), device=codes.device), scales.int() - 127))
+    s = torch.where(scales > 252, float("nan"), torch.ldexp(torch.ones((), device=codes.device), scales.int() - 127))
     return (x * s[..., None]).flatten(-2)
 
 

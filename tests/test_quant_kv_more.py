@@ -54,3 +54,33 @@ def check_loud(q, cache, table, ctx, q_start, attend):
 def test_values_at_the_end_of_the_range(lens):
     q, cache, table, ctx, q_start = t.attention_case("mxfp4", 64, 4, 2, 16, [120, 333], lens)
     check_loud(q, cache, table, ctx, q_start, lambda x: ops.quant_attention(x, cache, table, ctx, q_start))
+
+
+def check_bytes_of_no_number(q, cache, table, ctx, q_start, attend, seq, seen_by):
+    """Exponent bytes of 253 to 255, of a block of a key and of a value of sequence ``seq``'s tokens 2 and 9: NaN to whoever reads the block, and to the rows (a mask [T]) that see the token."""
+    page, G, head = cache.k.shape[2], q.shape[1] // cache.heads, cache.heads - 1
+    want = attend(q)
+    assert not torch.isnan(want).any()
+    pos = t.ints([2, 9, 1]).to(q.device)
+    of = torch.full_like(pos, seq)
+    for byte in (253, 254, 255):
+        for which, token, other in (("ks", 2, "vs"), ("vs", 9, "ks")):
+            place, scales = (int(table[seq, token // page]), head, token % page, 1), getattr(cache, which)
+            kept = int(scales[place])
+            scales[place] = byte
+            read = dict(zip(("ks", "vs"), ops.quant_kv_read(cache, table, pos, of)))
+            at = pos.tolist().index(token)
+            bad = torch.isnan(read[which])
+            assert bad[at, head, 32:64].all() and bad.sum() == 32 and not torch.isnan(read[other]).any()
+            out = attend(q)
+            bad = torch.isnan(out).cpu()
+            assert bad[:, G * head:][seen_by].all() and bad.sum() == G * q.shape[2] * int(seen_by.sum()), (byte, which)
+            scales[place] = kept
+    assert torch.equal(attend(q), want)
+
+
+def test_bytes_of_no_number():
+    q, cache, table, ctx, q_start = t.attention_case("mxfp4", 64, 4, 2, 16, [70, 33], [20, 33])
+    seen = torch.zeros(53, dtype=torch.bool)
+    seen[:20] = True
+    check_bytes_of_no_number(q, cache, table, ctx, q_start, lambda x: ops.quant_attention(x, cache, table, ctx, q_start), 0, seen)

@@ -60,3 +60,24 @@ def test_values_at_the_end_of_the_range(form, D):
 def test_values_at_the_end_of_the_range_in_a_prefix(form, D):
     q, cache, table, ctx, groups, prefix, q_start, wide = shared_case(form, "mxfp4", D)
     m.check_loud(q, cache, table, ctx, q_start, lambda x: ops.prefix_attention(x, cache, wide, ctx, groups, prefix, q_start))
+
+
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("form", OWN)
+def test_bytes_of_no_number(form, D):
+    q, cache, table, ctx, q_start, wide = own_case(form, "mxfp4", D)
+    start = list(range(len(ctx) + 1)) if q_start is None else q_start.tolist()
+    seen = torch.zeros(q.shape[0], dtype=torch.bool)
+    for i in range(start[0], start[1]):
+        seen[i] = int(ctx[0]) - start[1] + i >= 9
+    assert seen[start[0]:start[1]].all()                         # tokens 2 and 9 are before all of them
+    m.check_bytes_of_no_number(q, cache, table, ctx, q_start, lambda x: ops.quant_attention(x, cache, wide, ctx, q_start), 0, seen)
+
+
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("form", SHARED)
+def test_bytes_of_no_number_in_a_prefix(form, D):
+    q, cache, table, ctx, groups, prefix, q_start, wide = shared_case(form, "mxfp4", D)
+    seen = torch.zeros(q.shape[0], dtype=torch.bool)
+    seen[int(groups[0]):int(groups[1])] = True                   # the one group's rows, a token each
+    m.check_bytes_of_no_number(q, cache, table, ctx, q_start, lambda x: ops.prefix_attention(x, cache, wide, ctx, groups, prefix, q_start), int(groups[0]), seen)
