@@ -7,7 +7,7 @@
 // It reads T (Hq + 2 Hkv) D 2 bytes and writes T Hq D 2 and the rows' codes: bytes are what bounds it.  D / 8 lanes a head row, 16 bytes a lane; a lane's rotation
 // partner is D / 16 lanes away or none, and its eight numbers are read a second time (they are in the cache) where an exchange would go through LDS.  Keys and values
 // go by double up to their codes: a key next to a border between two codes then takes the code of the formula, whatever the order of sums, and it costs nothing beside
-// the bytes.  The queries, most of the rows, are float32 (all rows in double: 237 us for 16384 tokens of 64 + 16 heads of 128 in int8, against 133, 645 MB at 4.8 TB/s).
+// the bytes.  The queries, most of the rows, are float32, in a power of two's units where their squares would pass its range (all rows in double: 237 us for 16384 tokens of 64 + 16 heads of 128 in int8, against 133, 645 MB at 4.8 TB/s).
 #include "chronos_quant_kv.h"
 
 namespace chronos {
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(256) norm_rope_kv_quant_kernel(
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const u16x8 po = turns ? xp[i] : zero;
+            u16x8 po = turns ? xp[i] : zero;
             float x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = bf2f(xr[i][j]);
@@ -156,7 +156,19 @@ __global__ void __launch_bounds__(256) norm_rope_kv_quant_kernel(
                 float ss = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
-                f = rsqrtf(group_sum(ss, L) * (1.f / D) + (float)eps);
+                float m = group_sum(ss, L) * (1.f / D) + (float)eps;
+                if (!(m > 0x1p-100f && m < 0x1p100f)) {   // squares at the ends of float32's range: the row times a power of two, eps times its square
+                    const float by = m < 1.f ? 0x1p80f : 0x1p-80f;
+                    ss = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        x[j] *= by;
+                        po[j] = f2bf(bf2f(po[j]) * by);
+                        ss += x[j] * x[j];
+                    }
+                    m = group_sum(ss, L) * (1.f / D) + (float)(eps * by * by);
+                }
+                f = rsqrtf(m);
             }
             u16x8 o;
 #pragma unroll

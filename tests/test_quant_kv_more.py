@@ -84,3 +84,30 @@ def test_bytes_of_no_number():
     seen = torch.zeros(53, dtype=torch.bool)
     seen[:20] = True
     check_bytes_of_no_number(q, cache, table, ctx, q_start, lambda x: ops.quant_attention(x, cache, table, ctx, q_start), 0, seen)
+
+
+SIZES = (1.0, 1e30, 3e38, 1e-18, 1e-30, 1e-38)
+
+
+def check_norms(device, D, tokens, eps):
+    """Rows whose squares are no numbers of float32, and ordinary ones beside them: normed as others are."""
+    hq, hkv, page = 8, 2, 16
+    (qkv, pos, seq, table, cs, wq, wk), cache = t.write_case("int8", D, hq, hkv, page, D, True, [tokens], [tokens], device=device)
+    x = torch.randn(tokens, hq + 2 * hkv, D, generator=torch.Generator().manual_seed(9)).clamp(-1, 1)
+    x = (x * torch.tensor(SIZES)[torch.arange(tokens * (hq + 2 * hkv)).view(tokens, -1, 1) % len(SIZES)]).to(BF)
+    q = ops.norm_rope_kv_quant(x.flatten(1).to(device), pos, seq, table, cs, cache, hq, wq, wk, eps=eps)
+    want = plain.norm_rotation(x[:, :hq], wq.cpu(), eps, cs.cpu(), pos.cpu())
+    # Half a step of the output's type, and float32 products: relative to a row's largest.  bfloat16's numbers below 2^-126 are 2^-133 apart: rows of 1e-38 over 1e-3 have such
+    # numbers, whose half step is 2^-134 whatever their size.
+    assert ((q.double().cpu() - want).abs() <= t.HALF * want.abs() + 2 ** -20 * want.abs().amax(-1, keepdim=True) + 2 ** -134).all()
+    if eps == 0:
+        assert (want.abs().amax(-1) > 0.5).all()
+    codes, scales = plain.quantise(plain.norm_rotation(x[:, hq:hq + hkv], wk.cpu(), eps, cs.cpu(), pos.cpu()), "int8")
+    p, o = table.cpu()[0, torch.arange(tokens) // page].long(), torch.arange(tokens) % page
+    assert torch.equal(cache.k.cpu()[p, :, o].long(), codes) and torch.equal(cache.ks.cpu()[p, :, o], scales)
+
+
+@pytest.mark.parametrize("eps", (0.0, 1e-6))
+@pytest.mark.parametrize("D", (64, 128))
+def test_norms_of_large_and_small_rows(D, eps):
+    check_norms("cpu", D, 9, eps)

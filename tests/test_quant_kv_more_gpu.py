@@ -81,3 +81,10 @@ def test_bytes_of_no_number_in_a_prefix(form, D):
     seen = torch.zeros(q.shape[0], dtype=torch.bool)
     seen[int(groups[0]):int(groups[1])] = True                   # the one group's rows, a token each
     m.check_bytes_of_no_number(q, cache, table, ctx, q_start, lambda x: ops.prefix_attention(x, cache, wide, ctx, groups, prefix, q_start), int(groups[0]), seen)
+
+
+@pytest.mark.parametrize("eps", (0.0, 1e-6))
+@pytest.mark.parametrize("tokens", (9, 1030), ids=("a row a lane", "four"))
+@pytest.mark.parametrize("D", (64, 128))
+def test_norms_of_large_and_small_rows(D, tokens, eps):
+    m.check_norms(DEV, D, tokens, eps)
