@@ -111,3 +111,22 @@ def check_norms(device, D, tokens, eps):
 @pytest.mark.parametrize("D", (64, 128))
 def test_norms_of_large_and_small_rows(D, eps):
     check_norms("cpu", D, 9, eps)
+
+
+def check_equal_values(q, cache, table, ctx, q_start, attend):
+    """All of a head's values alike: rows that see any key have that value, whatever the scores.  Codes of seven bits at most and scales of powers of two: bfloat16 holds the value, and half a
+    step of it, 2^-9 of its size at least, is more than float16's rounding of the probabilities (2^-11 at most) and float32 sums of some 500 (2^-14) come to."""
+    cache.v.copy_(cache.v[0, :, :1].clone())
+    cache.vs.fill_(2.0 ** -3) if cache.kind == "int8" else cache.vs.fill_(124)
+    v = plain.values(cache)[1][0, :, 0].to(q.device)
+    start = list(range(len(ctx) + 1)) if q_start is None else q_start.tolist()
+    want = v.repeat_interleave(q.shape[1] // cache.heads, 0).expand(q.shape).clone()
+    want[start[-1]:] = 0
+    assert torch.equal(attend(q).double(), want)
+
+
+@pytest.mark.parametrize("kind", t.KINDS)
+@pytest.mark.parametrize("lens", (None, [40, 130]), ids=("rows", "prompts"))
+def test_equal_values(kind, lens):
+    q, cache, table, ctx, q_start = t.attention_case(kind, 64, 4, 2, 16, [120, 333], lens)
+    check_equal_values(q, cache, table, ctx, q_start, lambda x: ops.quant_attention(x, cache, table, ctx, q_start))

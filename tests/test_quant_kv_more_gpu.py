@@ -88,3 +88,19 @@ def test_bytes_of_no_number_in_a_prefix(form, D):
 @pytest.mark.parametrize("D", (64, 128))
 def test_norms_of_large_and_small_rows(D, tokens, eps):
     m.check_norms(DEV, D, tokens, eps)
+
+
+@pytest.mark.parametrize("kind", t.KINDS)
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("form", OWN)
+def test_equal_values(form, D, kind):
+    q, cache, table, ctx, q_start, wide = own_case(form, kind, D)
+    m.check_equal_values(q, cache, table, ctx, q_start, lambda x: ops.quant_attention(x, cache, wide, ctx, q_start))
+
+
+@pytest.mark.parametrize("kind", t.KINDS)
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("form", SHARED)
+def test_equal_values_in_a_prefix(form, D, kind):
+    q, cache, table, ctx, groups, prefix, q_start, wide = shared_case(form, kind, D)
+    m.check_equal_values(q, cache, table, ctx, q_start, lambda x: ops.prefix_attention(x, cache, wide, ctx, groups, prefix, q_start))
