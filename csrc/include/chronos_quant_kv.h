@@ -24,10 +24,11 @@ struct Cache {
 };
 
 // How a call of the attention is cut up (quant_attention.hip): rows of a tile, tiles and pieces of the keys, for the sequences' own keys and for those that
-// groups share; slots of partial sums, 1: none
+// groups share; slots of partial sums, 1: none; whether the launch over the own keys joins the groups' pieces itself, and whether it takes the tiles with most keys first
 struct AttnPlan {
     int own_rows, own_splits, group_rows, group_splits, slots;
     int64_t own_tiles, group_tiles;
+    bool last, longest;
 };
 
 template <int KIND, int D> constexpr int row_bytes() { return KIND == kInt8 ? D : D / 2; }

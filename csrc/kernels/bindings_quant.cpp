@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <tuple>
+#include <vector>
 
 #include "chronos_quant_kv.h"
 
@@ -170,6 +171,15 @@ Tensor quant_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
     return out;
 }
 
+// How quant_attention cuts a call up: rows of a tile of the sequences' own keys, pieces of those keys, rows and pieces of what groups share, and whether the own keys' launch joins the groups'
+// pieces and whether it takes its longest tiles first.  single: no q_start; keys: the table's width in keys, or max_ctx.
+std::vector<int64_t> quant_attention_plan(int64_t T, int64_t B, bool single, int64_t groups, int64_t hq, int64_t heads, int64_t keys) {
+    CHK(T > 0 && T < kMost && B > 0 && B < kMost && groups >= 0 && groups < kMost && keys > 0 && keys < kMost, "a plan needs tokens, sequences and keys");
+    CHK(heads > 0 && hq > 0 && hq < 65536 && hq % heads == 0, "q heads (", hq, ") must be a multiple of the cache's (", heads, ")");
+    const auto p = chronos::qkv::quant_attention_plan((int)T, (int)B, single, (int)groups, (int)hq, (int)heads, keys);
+    return {p.own_rows, p.own_splits, p.group_rows, p.group_splits, p.last, p.longest};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(chronos, m) {
@@ -178,6 +188,7 @@ TORCH_LIBRARY_FRAGMENT(chronos, m) {
     m.def("quant_kv_read(Tensor k, Tensor v, Tensor ks, Tensor vs, Tensor block_table, Tensor pos, Tensor tok_seq) -> (Tensor, Tensor)");
     m.def("quant_attention(Tensor q, Tensor k, Tensor v, Tensor ks, Tensor vs, Tensor block_table, Tensor ctx_len, Tensor? q_start, Tensor? group_start, "
           "Tensor? prefix_len, float scale, int max_ctx=-1) -> Tensor");
+    m.def("quant_attention_plan(int T, int B, bool single, int groups, int hq, int heads, int keys) -> int[]", &quant_attention_plan);
 }
 
 TORCH_LIBRARY_IMPL(chronos, CUDA, m) {

@@ -1202,6 +1202,9 @@ AttnPlan quant_attention_plan(int T, int B, bool single, int groups, int hq, int
     if (single) p.own_tiles = (int64_t)T * ((hq / heads + p.own_rows - 1) / p.own_rows);
     if (groups > 0) side(groups, false, p.group_rows, p.group_tiles, p.group_splits);
     p.slots = p.own_splits + p.group_splits;
+    p.last = groups > 0 && p.own_rows <= 32 && p.own_splits == 1;
+    // A tile of 256 rows has a CU for itself.  Prompts of up to 2048 tokens behind up to 2048 of context, two of them: 163 us so, 218 in order; 16 of up to 256: 64 and 66.
+    p.longest = !single && groups == 0 && B < 256 && p.own_rows == 256 && p.own_tiles * heads > 256;
     return p;
 }
 
@@ -1219,9 +1222,8 @@ void launch_quant_attention(int kind, int D, const AttnPlan& p, const uint16_t* 
     }
     a.splits = p.own_splits;
     a.slot0 = p.group_splits;
-    a.last = groups && p.own_rows <= 32 && p.own_splits == 1;
-    // A tile of 256 rows has a CU for itself.  Prompts of up to 2048 tokens behind up to 2048 of context, two of them: 163 us so, 218 in order; 16 of up to 256: 64 and 66.
-    a.longest = q_start && !groups && B < 256 && p.own_rows == 256 && p.own_tiles * cache.heads > 256;
+    a.last = p.last;
+    a.longest = p.longest;
     launch_rows_of<false>(kind, D, p.own_rows, a, p.own_tiles, st);
     if (p.slots > 1 && !a.last) {
         const int64_t rows = (int64_t)T * hq;

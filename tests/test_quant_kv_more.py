@@ -10,6 +10,63 @@ from tests.oracles import quant_kv_whole as whole
 BF = torch.bfloat16
 
 
+# The forms that attention's rules choose, and the plan that each has to have: rows of a tile of the sequences' own keys, pieces of those, the same of what groups share, whether the own keys'
+# launch joins the groups' pieces, whether it takes its longest tiles first.
+# Of own keys: (hq, hkv, page, contexts, tokens, keys that the table has room for at least, plan)
+OWN = {
+    "16 rows": (8, 2, 16, [500, 33, 200], None, 0, (16, 1, 0, 0, False, False)),
+    "16 rows, pieces": (8, 2, 16, [1500, 700], None, 0, (16, 6, 0, 0, False, False)),
+    "32 rows": (64, 32, 16, [90, 40, 130], [60, 20, 60], 0, (32, 1, 0, 0, False, False)),
+    "32 rows, pieces": (64, 32, 16, [390, 40, 530], [60, 20, 60], 5000, (32, 3, 0, 0, False, False)),
+    "256 rows": (64, 64, 16, [300, 200], [150, 112], 0, (256, 1, 0, 0, False, False)),
+    "256 rows, pieces": (64, 64, 16, [300, 200], [150, 112], 2048, (256, 2, 0, 0, False, False)),
+    "256 rows, longest first": (64, 64, 16, [300, 140, 200], [150, 140, 100], 0, (256, 1, 0, 0, False, True)),
+    # more sequences than a wave has lanes, lengths far apart, some without a token, some with more tokens than context; as many as there may be
+    "70 sequences, longest first": (64, 4, 16, [5, 60] + [(37 * i) % 170 + 1 for i in range(68)], [9, 60] + [(13 * i) % 17 for i in range(68)], 0, (256, 1, 0, 0, False, True)),
+    "255 sequences, longest first": (16, 1, 32, [(53 * i) % 190 for i in range(255)], [(29 * i) % 16 for i in range(255)], 0, (256, 1, 0, 0, False, True)),
+}
+# Of what groups share: (hq, hkv, page, shared pages of each group, sequences of each, own tokens, tokens of each, sequences before and behind, keys that the table has room for, plan)
+SHARED = {
+    "16 rows": (8, 2, 16, [30], [6], [1, 20, 16, 33, 2, 40], None, 1, 0, (16, 1, 16, 9, True, False)),
+    "32 rows": (8, 1, 16, [30], [40], [1 + i % 29 for i in range(40)], None, 1, 0, (16, 1, 32, 4, True, False)),
+    "128 rows": (32, 16, 16, [20], [100], [1 + i % 29 for i in range(100)], None, 1, 0, (16, 1, 128, 2, True, False)),
+    "256 rows": (64, 32, 16, [20], [60], [1 + i % 29 for i in range(60)], None, 1, 0, (16, 1, 256, 2, True, False)),
+    # joined by a launch of its own: tables of more than 32768 keys, or own tiles of 256 rows; a group without pages, one of a single sequence
+    "16 rows, joined": (8, 2, 16, [30, 0, 5], [6, 3, 1], [1, 20, 16, 33, 2, 40, 9, 50, 17, 60], None, 2, 70000, (16, 3, 16, 51, False, False)),
+    "16 rows of some tokens, joined": (12, 2, 32, [9, 2], [4, 3], [40, 3, 160, 7, 1, 20, 90], [2, 1, 3, 3, 1, 0, 2], 1, 40000, (16, 2, 16, 36, False, False)),
+    "32 rows, joined": (8, 1, 16, [30], [40], [1 + i % 29 for i in range(40)], None, 1, 70000, (16, 3, 32, 42, False, False)),
+    "own 256 rows, joined": (32, 32, 16, [5, 2], [3, 1], [230, 200, 190, 205], [200, 190, 180, 150], 1, 0, (256, 1, 256, 2, False, False)),
+}
+
+
+def plan(T, B, single, groups, hq, hkv, keys):
+    ops.load()
+    p = torch.ops.chronos.quant_attention_plan(T, B, single, groups, hq, hkv, keys)
+    return (*p[:4], bool(p[4]), bool(p[5]))
+
+
+@pytest.mark.parametrize("form", OWN)
+def test_plans(form):
+    hq, hkv, page, ctx, lens, keys, want = OWN[form]
+    T = (len(ctx) if lens is None else sum(lens)) + 3
+    assert plan(T, len(ctx), lens is None, 0, hq, hkv, -(-max(max(ctx), keys) // page) * page) == want
+
+
+@pytest.mark.parametrize("form", SHARED)
+def test_shared_plans(form):
+    hq, hkv, page, pages, seqs, own, lens, more, keys, want = SHARED[form]
+    ctx = [50 + 7 * i for i in range(2 * more)] + [pages[g] * page + o for g, o in zip([g for g, n in enumerate(seqs) for _ in range(n)], own)]
+    T = (len(ctx) if lens is None else 3 * more + sum(lens)) + 3
+    assert plan(T, len(ctx), lens is None, len(seqs), hq, hkv, -(-max(max(ctx), keys) // page) * page) == want
+
+
+def test_plans_that_cannot_be():
+    ops.load()
+    for bad in ((0, 1, True, 0, 8, 2, 100), (1, 0, True, 0, 8, 2, 100), (1, 1, True, -1, 8, 2, 100), (1, 1, True, 0, 8, 3, 100), (1, 1, True, 0, 8, 0, 100), (1, 1, True, 0, 8, 2, 0)):
+        with pytest.raises(RuntimeError, match="chronos"):
+            torch.ops.chronos.quant_attention_plan(*bad)
+
+
 def check(out, q, cache, table, ctx, q_start=None, more=0.0):
     """:func:`test_quant_kv.check_attention`'s bound, against the oracle for many rows; ``more``: what else is off relative to sum_j p_j |v_j|."""
     want, size = whole.attention(q, cache, table, ctx, q_start)
@@ -121,6 +178,8 @@ def check_equal_values(q, cache, table, ctx, q_start, attend):
     v = plain.values(cache)[1][0, :, 0].to(q.device)
     start = list(range(len(ctx) + 1)) if q_start is None else q_start.tolist()
     want = v.repeat_interleave(q.shape[1] // cache.heads, 0).expand(q.shape).clone()
+    for b, c in enumerate(ctx.tolist()):
+        want[start[b]:min(start[b + 1], max(start[b], start[b + 1] - c))] = 0      # more tokens than context
     want[start[-1]:] = 0
     assert torch.equal(attend(q).double(), want)
 

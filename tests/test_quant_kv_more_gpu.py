@@ -11,23 +11,7 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda"
 cpu = g.cpu
 
-# Forms of a sequence's own keys: (hq, hkv, page, contexts, tokens, keys that the table has room for at least)
-OWN = {
-    "16 rows": (8, 2, 16, [500, 33, 200], None, 0),
-    "16 rows, pieces": (8, 2, 16, [1500, 700], None, 0),
-    "32 rows": (64, 32, 16, [90, 40, 130], [60, 20, 60], 0),
-    "32 rows, pieces": (64, 32, 16, [390, 40, 530], [60, 20, 60], 5000),
-    "256 rows": (64, 64, 16, [300, 200], [150, 112], 0),
-    "256 rows, pieces": (64, 64, 16, [300, 200], [150, 112], 2048),
-    "256 rows, longest first": (64, 64, 16, [300, 140, 200], [150, 140, 100], 0),
-}
-# and of what groups share: (hq, hkv, page, shared pages of each group, sequences of each, own tokens, tokens of each, sequences before and behind, keys that the table has room for)
-SHARED = {
-    "16 rows": (8, 2, 16, [30], [6], [1, 20, 16, 33, 2, 40], None, 1, 0),
-    "32 rows": (8, 1, 16, [30], [40], [1 + i % 29 for i in range(40)], None, 1, 0),
-    "128 rows": (32, 16, 16, [20], [100], [1 + i % 29 for i in range(100)], None, 1, 0),
-    "256 rows": (64, 32, 16, [20], [60], [1 + i % 29 for i in range(60)], None, 1, 0),
-}
+OWN, SHARED = m.OWN, m.SHARED
 
 
 def widened(table, keys, page):
@@ -37,15 +21,26 @@ def widened(table, keys, page):
 
 
 def own_case(form, kind, D):
-    hq, hkv, page, ctx, lens, keys = OWN[form]
+    """q, cache, table, ctx, q_start, the table as wide as the form asks; three rows behind the last sequence."""
+    hq, hkv, page, ctx, lens, keys, _ = OWN[form]
     q, cache, table, ctx, q_start = t.attention_case(kind, D, hq, hkv, page, ctx, lens, DEV, tail=3)
+    poison()
     return q, cache, table, ctx, q_start, widened(table, keys, page)
 
 
 def shared_case(form, kind, D):
-    *case, keys = SHARED[form]
+    """q, cache, table, ctx, groups, prefix, q_start, the wide table."""
+    *case, keys, _ = SHARED[form]
     (q, table, ctx, groups, prefix, q_start), cache = g.prefix_case(kind, D, *case)
+    q = torch.cat([q, t.rows_of(3, q.shape[1], D, 7).to(DEV)])
+    poison()
     return q, cache, table, ctx, groups, prefix, q_start, widened(table, keys, case[2])
+
+
+def poison():
+    """What the allocator hands out next holds NaN: partial sums that nobody wrote show."""
+    for n in (1 << 16, 1 << 20, 1 << 22, 1 << 24, 1 << 26):
+        torch.full((n,), float("nan"), device=DEV)
 
 
 @pytest.mark.parametrize("D", (64, 128))
@@ -67,11 +62,10 @@ def test_values_at_the_end_of_the_range_in_a_prefix(form, D):
 def test_bytes_of_no_number(form, D):
     q, cache, table, ctx, q_start, wide = own_case(form, "mxfp4", D)
     start = list(range(len(ctx) + 1)) if q_start is None else q_start.tolist()
+    seq = next(b for b, c in enumerate(ctx.tolist()) if start[b + 1] > start[b] and c - start[b + 1] + start[b] > 9)       # tokens 2 and 9 are before all of its rows
     seen = torch.zeros(q.shape[0], dtype=torch.bool)
-    for i in range(start[0], start[1]):
-        seen[i] = int(ctx[0]) - start[1] + i >= 9
-    assert seen[start[0]:start[1]].all()                         # tokens 2 and 9 are before all of them
-    m.check_bytes_of_no_number(q, cache, table, ctx, q_start, lambda x: ops.quant_attention(x, cache, wide, ctx, q_start), 0, seen)
+    seen[start[seq]:start[seq + 1]] = True
+    m.check_bytes_of_no_number(q, cache, table, ctx, q_start, lambda x: ops.quant_attention(x, cache, wide, ctx, q_start), seq, seen)
 
 
 @pytest.mark.parametrize("D", (64, 128))
@@ -79,7 +73,8 @@ def test_bytes_of_no_number(form, D):
 def test_bytes_of_no_number_in_a_prefix(form, D):
     q, cache, table, ctx, groups, prefix, q_start, wide = shared_case(form, "mxfp4", D)
     seen = torch.zeros(q.shape[0], dtype=torch.bool)
-    seen[int(groups[0]):int(groups[1])] = True                   # the one group's rows, a token each
+    start = list(range(len(ctx) + 1)) if q_start is None else q_start.tolist()
+    seen[start[int(groups[0])]:start[int(groups[1])]] = True      # the first group's rows: its shared pages hold tokens 2 and 9
     m.check_bytes_of_no_number(q, cache, table, ctx, q_start, lambda x: ops.prefix_attention(x, cache, wide, ctx, groups, prefix, q_start), int(groups[0]), seen)
 
 
@@ -104,3 +99,127 @@ def test_equal_values(form, D, kind):
 def test_equal_values_in_a_prefix(form, D, kind):
     q, cache, table, ctx, groups, prefix, q_start, wide = shared_case(form, kind, D)
     m.check_equal_values(q, cache, table, ctx, q_start, lambda x: ops.prefix_attention(x, cache, wide, ctx, groups, prefix, q_start))
+
+
+@pytest.mark.parametrize("kind", t.KINDS)
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("form", OWN)
+def test_forms(form, D, kind):
+    q, cache, table, ctx, q_start, wide = own_case(form, kind, D)
+    out = ops.quant_attention(q, cache, wide, ctx, q_start)
+    m.check(out, q, cache, table, ctx, q_start)
+    assert not out[-3:].any()
+    assert torch.equal(out, ops.quant_attention(q, cache, wide, ctx, q_start))
+
+
+@pytest.mark.parametrize("kind", t.KINDS)
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("form", SHARED)
+def test_shared_forms(form, D, kind):
+    q, cache, table, ctx, groups, prefix, q_start, wide = shared_case(form, kind, D)
+    out = ops.prefix_attention(q, cache, wide, ctx, groups, prefix, q_start)
+    m.check(out, q, cache, table, ctx, q_start)
+    assert not out[-3:].any()
+    assert torch.equal(out, ops.prefix_attention(q, cache, wide, ctx, groups, prefix, q_start))
+
+
+def holes(cache, table, ctx, rows):
+    """Of the sequences `rows`, whose first pages may be the same: a hole, a page behind the cache's last, no pages at all behind some; a key and a value of NaN, an infinite key."""
+    nan, inf = (float("nan"), float("inf")) if cache.kind == "int8" else (255, 255)
+    first, page = rows[0], cache.k.shape[2]
+    at = [i for i in range(-(-int(ctx[first]) // page)) if i * page < int(ctx[rows].min())]      # pages that all of them have
+    head, pages = cache.heads - 1, table[first].tolist()
+    cache.vs[pages[at[0]], head, 5] = nan
+    cache.ks[pages[at[-1]], 0, min(3, int(ctx[rows].min()) - 1 - at[-1] * page)] = nan
+    if len(at) > 4:
+        cache.ks[pages[at[4]], head, page - 1] = inf
+    if len(at) > 3:
+        table[rows, at[1]], table[rows, at[3]] = -1, cache.k.shape[0]
+
+
+@pytest.mark.parametrize("kind", t.KINDS)
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("form", OWN)
+def test_holes_and_not_numbers(form, D, kind):
+    q, cache, table, ctx, q_start, _ = own_case(form, kind, D)
+    alive = [b for b in range(len(ctx)) if int(ctx[b]) > 40]
+    holes(cache, table, ctx, alive[:1])
+    table[alive[1], 1:] = -(1 << 31)
+    if len(alive) > 3:
+        holes(cache, table, ctx, alive[-1:])
+    wide = widened(table, OWN[form][5], OWN[form][2])
+    out = ops.quant_attention(q, cache, wide, ctx, q_start)
+    m.check(out, q, cache, table, ctx, q_start)
+    assert torch.isnan(out).any() and not torch.isnan(out).all()
+
+
+@pytest.mark.parametrize("kind", t.KINDS)
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("form", SHARED)
+def test_holes_and_not_numbers_in_a_prefix(form, D, kind):
+    """And contexts that end inside the shared pages, at their end, or are less than nothing."""
+    q, cache, table, ctx, groups, prefix, q_start, _ = shared_case(form, kind, D)
+    page, a, e = SHARED[form][2], int(groups[0]), int(groups[1])
+    holes(cache, table, ctx, list(range(a, e)))
+    ctx[a] = int(prefix[0]) - 7
+    ctx[a + 1] = int(prefix[0])
+    ctx[e - 1] = -(1 << 31)
+    ctx[0] = 3
+    wide = widened(table, SHARED[form][8], page)
+    out = ops.prefix_attention(q, cache, wide, ctx, groups, prefix, q_start)
+    m.check(out, q, cache, table, ctx, q_start)
+    assert torch.isnan(out).any() and not torch.isnan(out).all()
+
+
+def scattered(cache, table):
+    """int8: value scales over 2^61, some of nothing, and keys that grow with their page's place, so that scores do all the way."""
+    at = torch.arange(cache.vs.numel(), device=DEV).view(cache.vs.shape)
+    cache.vs.mul_(torch.exp2(((at * 37) % 61 - 30).float()))
+    for p, i in {p: i for row in table.tolist() for i, p in enumerate(row) if i}.items():
+        cache.ks[p] *= min(1 + i, 27)
+        if i % 7 == 3:
+            cache.vs[p] = 0
+
+
+def check_scattered(out, q, cache, table, ctx, q_start):
+    """Scores of up to 30 * 27: off by 2^-11 * 27 < 2^-6 relative to the probabilities, and the roundings as ever.  Probabilities times scales are float16, the largest, W, of a row's piece at 2^7 or
+    more: each is off by up to half of float16's least step, 2^-25 = 2^-32 W, times a code of up to 127; the largest's row has a code of 127, so 127 W is no more than the largest of the row's
+    sizes.  1600 keys at most.  Where the largest probabilities are of keys whose values are nothing, what is left are probabilities that float32 may not hold: less than 2^-126 each, times
+    1600 < 2^11 values of less than 2^33, is less than 2^-82."""
+    want, size = m.whole.attention(q, cache, table, ctx, q_start)
+    least = 1600 * 2 ** -32 * size.amax(-1, keepdim=True)
+    assert ((out.double() - want).abs() <= t.HALF * want.abs() + (t.HALF + 2 ** -6) * size + least + 2 ** -82).all()
+
+
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("form", OWN)
+def test_scales_far_apart(form, D):
+    q, cache, table, ctx, q_start, wide = own_case(form, "int8", D)
+    scattered(cache, table)
+    check_scattered(ops.quant_attention(q, cache, wide, ctx, q_start), q, cache, table, ctx, q_start)
+    cache.vs.fill_(0)
+    assert not ops.quant_attention(q, cache, wide, ctx, q_start).any()
+
+
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("form", SHARED)
+def test_scales_far_apart_in_a_prefix(form, D):
+    q, cache, table, ctx, groups, prefix, q_start, wide = shared_case(form, "int8", D)
+    scattered(cache, table)
+    check_scattered(ops.prefix_attention(q, cache, wide, ctx, groups, prefix, q_start), q, cache, table, ctx, q_start)
+    cache.vs.fill_(0)
+    assert not ops.prefix_attention(q, cache, wide, ctx, groups, prefix, q_start).any()
+
+
+@pytest.mark.parametrize("kind,D", (("int8", 128), ("mxfp4", 64)))
+def test_many_pieces_of_many_rows(kind, D):
+    """64 pieces of 32768 rows, which the joining launch takes in more than one turn: a table of 2^21 keys, the same for all sequences but for its first page."""
+    B, page = 2048, 1024
+    assert m.plan(B, B, True, 0, 16, 1, 1 << 21) == (16, 64, 0, 0, False, False)
+    cache = t.filled(17, page, 1, D, kind, DEV)
+    table = torch.arange(1 << 11, dtype=torch.int32, device=DEV).expand(B, -1) % 17
+    ctx = torch.tensor([(37 * i) % 300 if i % 100 else 9000 + 50 * i for i in range(B)], dtype=torch.int32, device=DEV).clamp(max=17 * page)
+    q = t.rows_of(B, 16, D).mul(2).to(DEV)
+    poison()
+    out = ops.quant_attention(q, cache, table, ctx)
+    m.check(out, q, cache, table, ctx)
