@@ -9,6 +9,8 @@
 //           values the error is .112 of their size, .115 with 6 or 8 in its place.
 //   A row (token, head) that holds an infinity or a NaN is held as NaN as a whole: scale NaN, E = 255 in all its blocks.  253 and 254, which no write makes, are read as 255
 //   is: six of their units pass float32's range.
+//   Attention keeps its accuracy for values between 2^-76 and 2^108 in int8, and up to the end of the range in mxfp4; smaller ones are written and read back as ever, but attention may
+//   give zeros for them.  Scores have to be numbers of float32.
 #pragma once
 #include "chronos_hip.h"
 

@@ -12,7 +12,8 @@
 //     same D / 16 neighbouring bytes of its eight keys, for all products, and no exchange between lanes.
 // int8: a key's scale multiplies its scores, a value's the probabilities.  These are then rounded to float16 (2^-11): in bfloat16 the largest probability of a row, 1 times a scale, would
 // be off by up to 2^-8 where without scales it is exact (.0025 of the output's size in place of .0017, of which its own rounding is .0016).  Each row's sums have a reference
-// that keeps its products in float16's range, the largest at 2^7 to 2^15, whatever the scales are; what is 2^-32 of the largest and less may get lost.
+// that keeps its products in float16's range, the largest at 2^7 to 2^15; what is 2^-32 of the largest and less may get lost.  That holds for value scales of 2^-83 to 2^101: probabilities are
+// float32 and go up to 2^90, so that they can be summed, and no lower than 2^-126, so beside smaller or larger scales less than 2^-32 gets lost, and all at 2^-115.
 // mxfp4: the conversion takes the scale, so a key's 32-dimension blocks have scales of their own that no probability can carry, and only bfloat16 has room for them: probabilities are bfloat16
 // (2^-8).  The sum that divides is of the rounded ones: what all of a row's large probabilities are off by in common then cancels, and an average of equal values is that value.  2 x 128 rows
 // of 64 heads on 16k shared keys: .0019 of the output's size, no number off by more than .0083, 189 us; with a sum of the unrounded .0020, .0119, 186 us.  The output's rounding alone is .00165 and .0078.

@@ -223,3 +223,16 @@ def test_many_pieces_of_many_rows(kind, D):
     poison()
     out = ops.quant_attention(q, cache, table, ctx)
     m.check(out, q, cache, table, ctx)
+
+
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("power", (-77, 105))
+@pytest.mark.parametrize("form", ("16 rows", "32 rows, pieces", "256 rows, pieces"))
+def test_ends_of_the_value_scales(form, power, D):
+    """int8 values of about 1 times 2^-77 and 2^105, scales of 2^-83 and 2^101: no less is lost than elsewhere, 2^-32 of a row's largest of each of 1600 keys at most."""
+    q, cache, table, ctx, q_start, wide = own_case(form, "int8", D)
+    cache.vs.mul_(2.0 ** power)
+    out = ops.quant_attention(q, cache, wide, ctx, q_start)
+    want, size = m.whole.attention(q, cache, table, ctx, q_start)
+    least = 1600 * 2 ** -32 * size.amax(-1, keepdim=True)
+    assert ((out.double() - want).abs() <= t.HALF * want.abs() + (t.HALF + 2 ** -10) * size + least).all() and out[:-3].any()
