@@ -117,10 +117,7 @@ def norm_rope_kv_quant(qkv: torch.Tensor, pos: torch.Tensor, tok_seq: torch.Tens
     row ``pos % page`` of page ``block_table[tok_seq, pos // page]``.  Returns the queries [T, hq, D].  Two tokens of one call must not have the same place.  The
     queries of a token without a place are zeros."""
     if _pkg._checking(qkv):
-        p, s, bt = pos.cpu().long(), tok_seq.cpu().long(), block_table.cpu().long()
-        ok, blk, row = ref.places(cache, bt, p, s)
-        _pkg._need(bool((p < cos_sin.shape[0]).all()), "norm_rope_kv_quant: position outside the rope table")
-        _pkg._need(bool((s < bt.shape[0]).all()) and bool((p < bt.shape[1] * cache.k.shape[2]).all()), "norm_rope_kv_quant: token outside the block table")
+        ok, blk, row = ref.places(cache, block_table.cpu(), pos.cpu(), tok_seq.cpu(), cos_sin.shape[0])      # tokens without a place are left out
         n = (blk * cache.k.shape[2] + row)[ok]
         _pkg._need(torch.unique(n).numel() == n.numel(), "norm_rope_kv_quant: two tokens in one place")
     if qkv.is_cuda:
@@ -181,7 +178,7 @@ def _attention(q, cache, block_table, ctx_len, q_start, group_start, prefix_len,
             gs, bt = group_start.cpu().long()[:prefix_len.numel() + 1], block_table.cpu()
             _pkg._need(bool((gs.diff() >= 0).all()) and int(gs[0]) >= 0 and int(gs[-1]) <= B, "prefix_attention: group_start")
             for g, n in enumerate(prefix_len.tolist()):
-                rows = bt[int(gs[g]):int(gs[g + 1]), :n // cache.k.shape[2]]
+                rows = bt[int(gs[g]):int(gs[g + 1]), :max(n, 0) // cache.k.shape[2]]
                 _pkg._need(bool((rows == rows[:1]).all()), f"prefix_attention: the pages of group {g} differ")
     if q.is_cuda:
         return _k("quant_attention")(q, cache.k, cache.v, cache.ks, cache.vs, block_table, ctx_len, q_start, group_start, prefix_len, scale, max_ctx)

@@ -189,3 +189,25 @@ def check_equal_values(q, cache, table, ctx, q_start, attend):
 def test_equal_values(kind, lens):
     q, cache, table, ctx, q_start = t.attention_case(kind, 64, 4, 2, 16, [120, 333], lens)
     check_equal_values(q, cache, table, ctx, q_start, lambda x: ops.quant_attention(x, cache, table, ctx, q_start))
+
+
+def check_checked(device):
+    """With inputs checked: what the documentation leaves out is left out as ever, what it rules out is named."""
+    for kind in t.KINDS:
+        t.check_left_out(kind, device)
+    (qkv, pos, seq, table, cs, wq, wk), cache = t.write_case("int8", 64, 2, 1, 16, 64, True, [4], [20], device=device)
+    padded, ones = t.ints([17, -1, -1, 18]).to(device), torch.zeros_like(seq)
+    ops.norm_rope_kv_quant(qkv, padded, ones, table, cs, cache, 2, wq, wk)
+    ops.norm_rope_kv_quant(qkv, t.ints([17, 19, 19, 18]).to(device), ones, table, cs[:19].contiguous(), cache, 2, wq, wk)      # both 19s are behind the rope table
+    with pytest.raises(IndexError, match="two tokens in one place"):
+        ops.norm_rope_kv_quant(qkv, t.ints([17, 18, 3, 18]).to(device), ones, table, cs, cache, 2, wq, wk)
+    q, cache, table, ctx, _ = t.attention_case("int8", 64, 2, 1, 16, [40, 70], None, device)
+    want, groups = ops.quant_attention(q, cache, table, ctx), t.ints([0, 2]).to(device)
+    assert torch.equal(ops.prefix_attention(q, cache, table, ctx, groups, t.ints([-1]).to(device)).isnan(), want.isnan())      # nothing shared
+    with pytest.raises(IndexError, match="pages of group 0 differ"):
+        ops.prefix_attention(q, cache, table, ctx, groups, t.ints([16]).to(device))
+
+
+def test_checked_inputs(monkeypatch):
+    monkeypatch.setattr(ops.quant_kv._pkg, "_checking", lambda x: True)
+    check_checked("cpu")

@@ -236,3 +236,11 @@ def test_ends_of_the_value_scales(form, power, D):
     want, size = m.whole.attention(q, cache, table, ctx, q_start)
     least = 1600 * 2 ** -32 * size.amax(-1, keepdim=True)
     assert ((out.double() - want).abs() <= t.HALF * want.abs() + (t.HALF + 2 ** -10) * size + least).all() and out[:-3].any()
+
+
+def test_checked_inputs():
+    ops.set_input_checks(True)
+    try:
+        m.check_checked(DEV)
+    finally:
+        ops.set_input_checks(False)
