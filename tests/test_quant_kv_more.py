@@ -45,28 +45,6 @@ def plan(T, B, single, groups, hq, hkv, keys):
     return (*p[:4], bool(p[4]), bool(p[5]))
 
 
-@pytest.mark.parametrize("form", OWN)
-def test_plans(form):
-    hq, hkv, page, ctx, lens, keys, want = OWN[form]
-    T = (len(ctx) if lens is None else sum(lens)) + 3
-    assert plan(T, len(ctx), lens is None, 0, hq, hkv, -(-max(max(ctx), keys) // page) * page) == want
-
-
-@pytest.mark.parametrize("form", SHARED)
-def test_shared_plans(form):
-    hq, hkv, page, pages, seqs, own, lens, more, keys, want = SHARED[form]
-    ctx = [50 + 7 * i for i in range(2 * more)] + [pages[g] * page + o for g, o in zip([g for g, n in enumerate(seqs) for _ in range(n)], own)]
-    T = (len(ctx) if lens is None else 3 * more + sum(lens)) + 3
-    assert plan(T, len(ctx), lens is None, len(seqs), hq, hkv, -(-max(max(ctx), keys) // page) * page) == want
-
-
-def test_plans_that_cannot_be():
-    ops.load()
-    for bad in ((0, 1, True, 0, 8, 2, 100), (1, 0, True, 0, 8, 2, 100), (1, 1, True, -1, 8, 2, 100), (1, 1, True, 0, 8, 3, 100), (1, 1, True, 0, 8, 0, 100), (1, 1, True, 0, 8, 2, 0)):
-        with pytest.raises(RuntimeError, match="chronos"):
-            torch.ops.chronos.quant_attention_plan(*bad)
-
-
 def check(out, q, cache, table, ctx, q_start=None, more=0.0):
     """:func:`test_quant_kv.check_attention`'s bound, against the oracle for many rows; ``more``: what else is off relative to sum_j p_j |v_j|."""
     want, size = whole.attention(q, cache, table, ctx, q_start)
@@ -211,3 +189,22 @@ def check_checked(device):
 def test_checked_inputs(monkeypatch):
     monkeypatch.setattr(ops.quant_kv._pkg, "_checking", lambda x: True)
     check_checked("cpu")
+
+
+def check_one_norm(device, four):
+    """Weights for the queries alone, and for the keys alone."""
+    case = ("mxfp4", 128, 8, 2, 16, 64, True, [1030 if four else 5], [1040 if four else 20])
+    for which in (0, 1):
+        (qkv, pos, seq, table, cs, wq, wk), cache = t.write_case(*case, device=device)
+        wq, wk = (wq, None) if which == 0 else (None, wk)
+        q = ops.norm_rope_kv_quant(qkv, pos, seq, table, cs, cache, 8, wq, wk)
+        x = qkv.cpu().view(len(pos), -1, 128)
+        want = plain.norm_rotation(x[:, :8], None if wq is None else wq.cpu(), 1e-6, cs.cpu(), pos.cpu())
+        assert ((q.double().cpu() - want).abs() <= t.HALF * want.abs() + 2 ** -20 * want.abs().amax(-1, keepdim=True)).all()
+        p, o = table.cpu()[0, pos.cpu().long() // 16].long(), pos.cpu().long() % 16
+        codes, scales = plain.quantise(plain.norm_rotation(x[-9:, 8:10], None if wk is None else wk.cpu(), 1e-6, cs.cpu(), pos.cpu()[-9:]), "mxfp4")
+        assert torch.equal(plain.whole_codes(cache)[0][p, :, o][-9:], codes) and torch.equal(cache.ks.cpu()[p, :, o][-9:].long(), scales)
+
+
+def test_one_norm():
+    check_one_norm("cpu", False)

@@ -43,6 +43,28 @@ def poison():
         torch.full((n,), float("nan"), device=DEV)
 
 
+@pytest.mark.parametrize("form", OWN)
+def test_plans(form):
+    hq, hkv, page, ctx, lens, keys, want = OWN[form]
+    T = (len(ctx) if lens is None else sum(lens)) + 3
+    assert m.plan(T, len(ctx), lens is None, 0, hq, hkv, -(-max(max(ctx), keys) // page) * page) == want
+
+
+@pytest.mark.parametrize("form", SHARED)
+def test_shared_plans(form):
+    hq, hkv, page, pages, seqs, own, lens, more, keys, want = SHARED[form]
+    ctx = [50 + 7 * i for i in range(2 * more)] + [pages[g] * page + o for g, o in zip([g for g, n in enumerate(seqs) for _ in range(n)], own)]
+    T = (len(ctx) if lens is None else 3 * more + sum(lens)) + 3
+    assert m.plan(T, len(ctx), lens is None, len(seqs), hq, hkv, -(-max(max(ctx), keys) // page) * page) == want
+
+
+def test_plans_that_cannot_be():
+    ops.load()
+    for bad in ((0, 1, True, 0, 8, 2, 100), (1, 0, True, 0, 8, 2, 100), (1, 1, True, -1, 8, 2, 100), (1, 1, True, 0, 8, 3, 100), (1, 1, True, 0, 8, 0, 100), (1, 1, True, 0, 8, 2, 0)):
+        with pytest.raises(RuntimeError, match="chronos"):
+            torch.ops.chronos.quant_attention_plan(*bad)
+
+
 @pytest.mark.parametrize("D", (64, 128))
 @pytest.mark.parametrize("form", OWN)
 def test_values_at_the_end_of_the_range(form, D):
@@ -244,3 +266,53 @@ def test_checked_inputs():
         m.check_checked(DEV)
     finally:
         ops.set_input_checks(False)
+
+
+@pytest.mark.parametrize("four", (False, True), ids=("a row a lane", "four"))
+def test_one_norm(four):
+    m.check_one_norm(DEV, four)
+
+
+def test_forms_in_graphs():
+    """Every form captured, two graphs of it at a time; replays among eager work and other replays, on new inputs, every one against the eager result."""
+    for kind, D in (("int8", 128), ("mxfp4", 64)):
+        calls = []
+        for form in OWN:
+            q, cache, _, ctx, q_start, wide = own_case(form, kind, D)
+            calls.append((q, lambda q=q, c=cache, x=ctx, s=q_start, w=wide: ops.quant_attention(q, c, w, x, s)))
+        for form in SHARED:
+            q, cache, _, ctx, groups, prefix, q_start, wide = shared_case(form, kind, D)
+            calls.append((q, lambda q=q, c=cache, x=ctx, a=groups, p=prefix, s=q_start, w=wide: ops.prefix_attention(q, c, w, x, a, p, s)))
+        graphs = []
+        for q, call in calls + calls:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = call()
+            graphs.append((graph, out))
+        for turn in range(3):
+            poison()
+            for i, (q, _) in enumerate(calls):
+                q.copy_(t.rows_of(q.shape[0], q.shape[1], D, 100 * turn + i))
+            for graph, _ in graphs:
+                graph.replay()
+            torch.cuda.synchronize()
+            for i, (_, call) in enumerate(calls):
+                want = call()
+                assert torch.equal(graphs[i][1], want) and torch.equal(graphs[i + len(calls)][1], want), (turn, i)
+
+
+def test_forms_on_two_streams():
+    """Two calls of every form at once."""
+    streams = [torch.cuda.Stream() for _ in "ab"]
+    for form in SHARED:
+        cases = [shared_case(form, kind, 64) for kind in t.KINDS]
+        calls = [lambda c=c: ops.prefix_attention(c[0], c[1], c[7], c[3], c[4], c[5], c[6]) for c in cases]
+        want, got = [c() for c in calls], [[], []]
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        for _ in range(3):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[i].append(calls[i]())
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, w) for g_, w in zip(got, want) for x in g_), form
