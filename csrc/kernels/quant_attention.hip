@@ -423,8 +423,8 @@ template <int N> __device__ __forceinline__ float moved_ref(float& ref, float ba
 // ---- the tile -----------------------------------------------------------------------------------------------------------------------------------------
 // GROUPS: the items are groups of sequences, the keys those that each shares; otherwise sequences, their keys behind what they share.
 // ONCE: the codes are marked as read once.
-// Bound by the codes' bytes where keys are many (two sequences of 128k, 64 query heads, mxfp4: 285 MB in 55 us, 5.2 TB/s; the join behind it 5), by the chain of loads (length, page, codes)
-// and the waves' join where they are few (a sequence of 140 keys 6.8 us).
+// Bound by the codes' bytes where keys are many (two sequences of 128k, 64 query heads, mxfp4: 285 MB in 57 to 59 us, 4.9 TB/s; the join behind it 5), by the chain of loads (length, page, codes)
+// and, where keys are few, by that chain once a step, since a wave asks for a step's codes when the one before is done, and by the waves' join (a sequence of 140 keys, two steps of one wave: 6.7 us).
 template <int KIND, int D, int NQT, bool GROUPS, bool ONCE>
 __global__ void __launch_bounds__(256, NQT == 1 ? (KIND == kInt8 && D == 128 ? 3 : 4) : 2) quant_rows_kernel(const AttnArgs a) {
     constexpr int ROWS = 16 * NQT, NC = D / 32, ND = D / 16;
@@ -704,8 +704,8 @@ __global__ void __launch_bounds__(256, NQT == 1 ? (KIND == kInt8 && D == 128 ? 3
 // loaded a step earlier, into the buffer that is not being read; one barrier a step.  16 bytes behind every row keep its readers, 16 bytes a lane and a row
 // each, out of each other's banks.  v_mfma_f32_32x32x16: a lane has 16 of 32 keys of one row, and the probabilities are the second product's operand as they are, its values' keys in the same order
 // (4 h + (j & 3) + 8 (j >> 2) of 16).
-// Two prompts of 1950 tokens and two of 330 on up to 3296 keys, 32 query heads, int8, 113 GFLOP: 174 us, 650 TFLOP/s; 2 x 128 sequences of 64 query heads on 16k shared keys, mxfp4,
-// 137 GFLOP: 150 us, 920 TFLOP/s.  There matrix cores are busy 39 % of the time and vector ALUs 44 %, one after the other for the most part: priorities of waves, half of them a step's part
+// Two prompts of 1950 tokens and two of 330 on up to 3296 keys, 32 query heads, int8, 113 GFLOP: 175 us, 650 TFLOP/s, matrix cores busy 31 % of the time and vector ALUs 48 %; 2 x 128 sequences of 64 query heads on 16k
+// shared keys, mxfp4, 137 GFLOP: 158 to 164 us, 850 TFLOP/s, 37 % and 41 % (profiles/quant_kv_counters.txt).  One after the other for the most part: priorities of waves, half of them a step's part
 // late, products a part late beside the next probabilities (which spills), and reads from LDS further ahead all gain nothing or lose.
 template <int KIND, int D, int WAVES> struct TileStep {
     static constexpr int KT = 16 * WAVES, KS = 2 * D + 16, VS = 2 * KT + 16;   // bytes from key to key, and from dimension to dimension
@@ -1180,16 +1180,25 @@ AttnPlan quant_attention_plan(int T, int B, bool single, int groups, int hq, int
         int64_t s = full / wgs, least = 256;
         if (own) {
             const int64_t busy = rows > 16 * items ? 160 : 224;
-            // Pieces take a launch to join.  Without any, a wave has 1000 keys in 8 us (2 x 700 keys: 9 us, with pieces 11; 16 x 1024: 10 and 12).  From `busy` workgroups on the
-            // card is busy enough (8 key heads, int8: 32 sequences of 2048 25 us, in two pieces 28, four 29; 24 of 500 to 2048 in four 20, in one 23), but for contexts that may be
-            // long, of which one may be far longer than the others (32 of 2048 to 8192 in four pieces 81, in two 82; of 8192 each 98 and 95;
-            // 8 x 96 rows on 2000 in tiles of 32 31 in one piece, 37 in four).
+            // Pieces take a launch to join.  int8, 32 query and 8 key heads of 128, us in 1 / 2 / 4 / 8 / 16 pieces (mixed: lengths of a quarter of the keys to all):
+            //   few workgroups, as many pieces as fill the card: 1 x 2048 keys 21 / 16 / 12 / 11 / 11, 12 x 2048 23 / 18 / 17 / 17 / 20, 12 x 4096 42 / 28 / 25 / 24 / 27;
+            //   none for short keys: 4 x 768 10.7 / 11.5 / 11.3 / 11.2 / 11.4, 12 x 768 10.8 / 11.2 / 12.4 / 12.2 / 14, and over that 4 x 1280 15 / 13 / 11 / 11 / 11.5; with more than 96
+            //   workgroups 27 x 1280 17 / 20 / 21 / 23 / 28, 13 x 1280 16 / 15 / 15 / 16 / 18, and over that 13 x 2048 23 / 19 / 17 / 20 / 21;
+            //   768 / workgroups from there to `busy`: 13 x 4096 42 / 28 / 25 / 28 / 27, 20 x 2048 24 / 24 / 23 / 23 / 27, mixed 23 / 22 / 20 / 21 / 25;
+            //   from `busy` on none: 27 x 2048 25 / 26 / 28 / 29 / 34, mixed 23 / 21 / 22 / 24 / 29, 28 x 2048 25 / 26 / 28 / 30 / 34, mixed 24 / 24 / 25 / 27 / 32; in tiles of 32 rows, which do more with
+            //   a key, sooner: 4 x 64 rows on 2000 31 / 34 / 40 / 55, 8 x 64 45 / 56 / 70 / 99;
+            //   but for contexts that may be long, of which one may be far longer than the others: 28 x 4096 52 / 49 / 51 / 52 / 60, mixed 51 / 44 / 40 / 40 / 47, 63 x 4096 91 / 98 / 103 / 114 /
+            //   129, mixed 89 / 93 / 78 / 82 / 93;
+            //   tiles of 256, a workgroup a CU: 1 x 1024 rows on 4096 146 / 100 / 110 in 1 / 2 / 4, 1 x 2048 on 4096 157 / 160 / 197; 20 x 32 on 2000, which get two, 72 / 87 / 84.
+            // For the most keys of a piece: 1 x 65536 in 8 / 16 / 32 / 64 81 / 46 / 30 / 31, 2 x 131072 186 / 108 / 97 / 101, 64 x 16384 in 1 / 2 / 4 / 8 352 / 359 / 358 / 370, mixed 316 / 306 / 301 / 290.
             if (tile == 256) s = (full + wgs / 2) / wgs;
             else if (wgs > 96) s = wgs < busy ? 768 / wgs : keys >= 4096 ? 1024 / wgs : 1;
             const int64_t longest = wgs < full ? 4096 : 16 * wgs;   // of a piece; the more there is beside it the longer one may take
             if (tile < 256 && keys / longest > s) s = keys / longest;
             if (keys <= (wgs > 96 ? 1280 : 768)) s = 1;
-            if (groups > 0) least = 32768;   // what sequences have of their own behind a shared prefix is taken to be short
+            // What sequences have of their own behind a shared prefix is taken to be short: in 1 / 4 / 8 / 16 pieces 64 sequences of 120 keys behind 2048 26 / 36 / 45 / 60 us, 16 of 1000 28 / 25 / 27 /
+            // 30.  Where it is long, this loses: 8 of 4000 53 / 30 / 29 / 30, two of 18000 (64 query heads) 175 / 59 / 39 / 30.
+            if (groups > 0) least = 32768;
         } else if (tile <= 32) {
             least = 4 * tile;   // 9 sequences on 480 shared keys: 13.5 us in pieces of 64, 17 in ones of 256
             const int64_t most = keys / 512 > 16 ? keys / 512 : 16;   // those behind wait for the sums: 16 sequences on 2048, one key head, in 16 pieces 16 us, in 32 18
